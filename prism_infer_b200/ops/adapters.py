@@ -1,0 +1,226 @@
+"""Low-rank adapters of many requests beside a shared projection.
+
+``y_t = W x_t + bias + scale_a B_a (A_a x_t)``, ``a`` the adapter of token ``t``.  ``W`` may stack several matrices by rows (query, key
+and value; gate and up): each of these sections has factors of its own.  An ``AdapterPool`` holds the factors of one projection for all
+loaded adapters, ``plan`` sorts out once per step which adapters its tokens use, ``linear`` and ``gate_up_glu`` are ``ops.linear`` and
+``ops.gate_up_glu`` with them.
+
+CUDA tensors run ``csrc/adapters.cu`` beside the GEMM kernels; CPU tensors the plain-PyTorch statement.
+"""
+
+from __future__ import annotations
+
+import ctypes
+from dataclasses import dataclass
+from typing import Optional, Sequence, Union
+
+import torch
+import torch.nn.functional as F
+
+from . import GLU_ACTS, _p, _pdl, _s, glu_act, native
+from .batch import check_device
+
+PANEL = 16             # ranks are padded to multiples of this
+TILE_TOKENS = 256      # tokens that share a list of adapters
+MAX_SLOTS = 8192
+MAX_SECTIONS = 8
+MAX_RANK = 256
+
+
+class AdapterPool:
+    """Factors of one projection ``[sum(sections), in_features]`` for up to ``slots`` adapters of rank up to ``rank`` per section, laid
+    out as the kernels read them: ``a [slots, sections * panels * 16, in_features]``, ``b [slots, panels, features, 16]``,
+    ``scale [slots]``.  A slot that was never loaded adds nothing."""
+
+    def __init__(self, slots: int, rank: int, in_features: int, sections: Union[int, Sequence[int]], *, device,
+                 dtype: torch.dtype = torch.bfloat16):
+        sections = (sections,) if isinstance(sections, int) else tuple(int(m) for m in sections)
+        if dtype not in (torch.bfloat16, torch.float32):
+            raise ValueError(f"adapters are bf16 or fp32, not {dtype}")
+        if not 1 <= slots <= MAX_SLOTS or not 1 <= rank <= MAX_RANK:
+            raise ValueError(f"{slots} slots of rank {rank}: at most {MAX_SLOTS} of rank {MAX_RANK}")
+        if not 1 <= len(sections) <= MAX_SECTIONS or min(sections) < 1 or in_features < 1:
+            raise ValueError(f"sections {sections} over {in_features} features: one to {MAX_SECTIONS} sections of at least one feature")
+        if dtype == torch.bfloat16 and in_features % 8:
+            raise ValueError(f"{in_features} input features: a bf16 row must be whole 16-byte vectors")
+        self.slots, self.rank, self.in_features, self.sections, self.dtype = slots, rank, in_features, sections, dtype
+        self.features = sum(sections)
+        self.panels = -(-rank // PANEL)
+        self.low = len(sections) * self.panels * PANEL
+        if slots * self.low >= 2 ** 31 or slots * self.panels * self.features >= 2 ** 31:
+            raise ValueError("the pool's rows must fit 31 bits")
+        self.a = torch.zeros(slots, self.low, in_features, dtype=dtype, device=device)
+        self.b = torch.zeros(slots, self.panels, self.features, PANEL, dtype=dtype, device=device)
+        self.scale = torch.zeros(slots, dtype=torch.float32, device=device)
+        self.device = self.a.device
+        ends = [sum(sections[:i + 1]) for i in range(len(sections))]
+        self._ends = (ctypes.c_int * len(ends))(*ends)
+
+    def load(self, slot: int, a, b, scale: float = 1.0) -> None:
+        """``a``: ``[r, in_features]`` and ``b``: ``[features, r]``, or one of each per section; ranks up to the pool's.  The copies are
+        made on the current stream.  Factors that are not finite are refused: tokens of other adapters meet them as products with
+        zero."""
+        a, b = ([f] if isinstance(f, torch.Tensor) else list(f) for f in (a, b))
+        if not 0 <= slot < self.slots:
+            raise ValueError(f"slot {slot} of {self.slots}")
+        if len(a) != len(self.sections) or len(b) != len(self.sections):
+            raise ValueError(f"{len(a)} and {len(b)} factors for {len(self.sections)} sections")
+        for fa, fb, m in zip(a, b, self.sections):
+            if fa.dim() != 2 or fb.dim() != 2 or fa.shape[1] != self.in_features or fb.shape[0] != m or fa.shape[0] != fb.shape[1]:
+                raise ValueError(f"factors {tuple(fa.shape)} and {tuple(fb.shape)} for {self.in_features} -> {m}")
+            if not 1 <= fa.shape[0] <= self.rank:
+                raise ValueError(f"rank {fa.shape[0]}, the pool holds up to {self.rank}")
+        scale = float(scale)
+        if not torch.isfinite(torch.tensor(scale, dtype=torch.float32)) or not all(bool(torch.isfinite(f.to(self.dtype)).all()) for f in (*a, *b)):
+            raise ValueError("factors and scale must be finite")
+        self.clear(slot)
+        first = 0
+        for i, (fa, fb, m) in enumerate(zip(a, b, self.sections)):
+            r, row = fa.shape[0], i * self.panels * PANEL
+            self.a[slot, row:row + r] = fa
+            padded = torch.zeros(m, self.panels * PANEL, dtype=self.dtype, device=self.device)
+            padded[:, :r] = fb
+            self.b[slot, :, first:first + m] = padded.view(m, self.panels, PANEL).transpose(0, 1)
+            first += m
+        self.scale[slot] = scale
+
+    def clear(self, slot: int) -> None:
+        """The slot adds nothing from here on."""
+        if not 0 <= slot < self.slots:
+            raise ValueError(f"slot {slot} of {self.slots}")
+        self.a[slot] = 0
+        self.b[slot] = 0
+        self.scale[slot] = 0
+
+
+@dataclass
+class AdapterPlan:
+    """``adapter [T]``: slot of every token, negative for none; per tile of 256 tokens the slots in use, ascending
+    (``lists [tiles, capacity]``, -1 behind), their number (``counts [tiles]``); ``index [T]``: a token's place in its tile's list."""
+
+    adapter: torch.Tensor
+    slots: int
+    index: torch.Tensor
+    lists: torch.Tensor
+    counts: torch.Tensor
+
+
+def plan(adapter: torch.Tensor, slots: int) -> AdapterPlan:
+    """Once per step, for every projection whose pool has ``slots`` slots.  ``adapter``: contiguous int32, one per token.  Slots out of
+    range count as none and set the ``adapters`` status word (``native.check_status``); on CPU they raise."""
+    if adapter.dtype != torch.int32 or adapter.dim() != 1 or not adapter.is_contiguous():
+        raise ValueError("adapter must be a contiguous one-dimensional int32 tensor")
+    if not 1 <= slots <= MAX_SLOTS:
+        raise ValueError(f"{slots} slots, one to {MAX_SLOTS}")
+    T = adapter.shape[0]
+    if T >= 2 ** 31 - TILE_TOKENS:
+        raise ValueError(f"{T} tokens")
+    tiles, capacity = -(-T // TILE_TOKENS), min(slots, TILE_TOKENS, T)
+    if not adapter.is_cuda:
+        if T and int(adapter.max()) >= slots:
+            raise ValueError(f"adapter {int(adapter.max())} of {slots} slots")
+        index, lists, counts = torch.full((T,), -1, dtype=torch.int32), torch.full((tiles, capacity), -1, dtype=torch.int32), torch.zeros(tiles, dtype=torch.int32)
+        for i in range(tiles):
+            who = adapter[i * TILE_TOKENS:(i + 1) * TILE_TOKENS]
+            used = torch.unique(who[who >= 0])
+            lists[i, :len(used)] = used
+            counts[i] = len(used)
+            index[i * TILE_TOKENS:(i + 1) * TILE_TOKENS] = torch.where(who >= 0, torch.searchsorted(used, who).int(), -1)
+        return AdapterPlan(adapter, slots, index, lists, counts)
+    check_device(adapter)
+    index, _, lists, _, counts = torch.empty(T + -T % 4 + tiles * capacity + -(tiles * capacity) % 4 + tiles, dtype=torch.int32, device=adapter.device).split(
+        (T, -T % 4, tiles * capacity, -(tiles * capacity) % 4, tiles))
+    if T:
+        native.call("prism_adapter_plan", _p(adapter), T, slots, capacity, _p(index), _p(lists), _p(counts), _s(), _pdl())
+    return AdapterPlan(adapter, slots, index, lists.view(tiles, capacity), counts)
+
+
+def _ld(t: torch.Tensor) -> int:
+    """Row stride; a single row may have any."""
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _check(x: torch.Tensor, w: torch.Tensor, pool: AdapterPool, p: AdapterPlan, bias: Optional[torch.Tensor], out: Optional[torch.Tensor],
+           features: int) -> None:
+    if x.dim() != 2 or w.dim() != 2 or x.shape[1] != pool.in_features or tuple(w.shape) != (pool.features, pool.in_features):
+        raise ValueError(f"x {tuple(x.shape)} and w {tuple(w.shape)} for a pool of {pool.in_features} -> {pool.features}")
+    tensors = [x, w] + [t for t in (bias, out) if t is not None]
+    if any(t.dtype != pool.dtype or t.device != pool.device for t in tensors) or p.adapter.device != pool.device:
+        raise ValueError(f"tensors must be {pool.dtype} on {pool.device}, as the pool is")
+    if p.slots != pool.slots or p.adapter.shape[0] != x.shape[0]:
+        raise ValueError(f"a plan of {p.adapter.shape[0]} tokens over {p.slots} slots for {x.shape[0]} tokens and {pool.slots} slots")
+    if bias is not None and (tuple(bias.shape) != (pool.features,) or not bias.is_contiguous()):
+        raise ValueError(f"bias must be contiguous, one value for each of {pool.features} features")
+    if out is not None and (tuple(out.shape) != (x.shape[0], features) or (features > 1 and out.stride(1) != 1) or _ld(out) < features):
+        raise ValueError(f"out must have shape {(x.shape[0], features)} and contiguous rows that are apart")
+    for name, t in (("x", x), ("w", w)):
+        ld = _ld(t)
+        if t.stride(1) != 1 or ld < t.shape[1] or (t.dtype == torch.bfloat16 and (ld % 8 or t.data_ptr() % 16)):
+            raise ValueError(f"{name}: rows must be contiguous and apart, in bf16 on 16-byte boundaries")
+    check_device(x)
+
+
+def _adapted_cpu(x, w, pool, p, bias):
+    y = F.linear(x.float(), w.float())
+    if bias is not None:
+        y += bias.float()
+    for s in torch.unique(p.adapter[p.adapter >= 0]).tolist():
+        rows = (p.adapter == s).nonzero()[:, 0]
+        low = F.linear(x[rows].float(), pool.a[s].float()) * pool.scale[s]
+        first, r = 0, pool.panels * PANEL
+        for i, m in enumerate(pool.sections):
+            b = pool.b[s, :, first:first + m].transpose(0, 1).reshape(m, r).float()
+            y[rows, first:first + m] += F.linear(low[:, i * r:(i + 1) * r], b)
+            first += m
+    return y
+
+
+def _run(x, w, pool, p, bias, out, act):
+    T, f32 = x.shape[0], int(pool.dtype == torch.float32)
+    if T == 0:
+        return out
+    base = torch.empty(T, pool.features, dtype=torch.float32, device=x.device)
+    if f32:
+        native.call("prism_gemm_f32", _p(w), _p(x), _p(base), pool.features, T, pool.in_features, _ld(w), _ld(x), pool.features,
+                    None, 0, None, None, None, 0.0, _s(), _pdl())
+    else:
+        native.call("prism_gemm_wx", _p(w), _p(x), _p(base), pool.features, T, pool.in_features, _ld(w), _ld(x), pool.features,
+                    pool.features, None, None, 0, 0, 0, 0, 1, 1, 0, 0, 0, _s(), _pdl())
+    h = torch.empty(T, pool.low, dtype=torch.float32, device=x.device)
+    native.call("prism_adapter_shrink", f32, _p(x), _p(pool.a), _p(pool.scale), _p(p.adapter), _p(h), T, pool.in_features, pool.low, pool.slots,
+                _ld(x), _s(), _pdl())
+    native.call("prism_adapter_expand", f32, _p(base), _p(h), _p(pool.b), _p(bias), _p(p.adapter), _p(out), T, pool.features, pool.panels,
+                pool.slots, len(pool.sections), pool._ends, act, _ld(out), _s(), _pdl())
+    return out
+
+
+def linear(x: torch.Tensor, w: torch.Tensor, pool: AdapterPool, p: AdapterPlan, *, bias: Optional[torch.Tensor] = None,
+           out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``x @ w.T + bias`` and every token's adapter; x ``[T, K]``, w ``[M, K]`` -> ``[T, M]``, sums in 32 bits, rounded once.  ``out``
+    shares no memory with the inputs."""
+    _check(x, w, pool, p, bias, out, pool.features)
+    if not x.is_cuda:
+        y = _adapted_cpu(x, w, pool, p, bias).to(x.dtype)
+        return y if out is None else out.copy_(y)
+    if out is None:
+        out = torch.empty(x.shape[0], pool.features, dtype=x.dtype, device=x.device)
+    return _run(x, w, pool, p, bias, out, 0)
+
+
+def gate_up_glu(x: torch.Tensor, w_gate_up: torch.Tensor, pool: AdapterPool, p: AdapterPlan, act: str, *,
+                out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``act(gate) * up`` with ``w_gate_up = [Wg ; Wu]`` and the adapters of both (a pool of two equal sections); ``act`` is ``silu`` or
+    ``gelu_tanh``.  Sums, activation and product in 32 bits, rounded once."""
+    if act not in ("silu", "gelu_tanh"):
+        raise ValueError(f"act {act!r} is neither silu nor gelu_tanh")
+    if len(pool.sections) != 2 or pool.sections[0] != pool.sections[1]:
+        raise ValueError(f"a gated unit has two equal sections, the pool {pool.sections}")
+    half = pool.sections[0]
+    _check(x, w_gate_up, pool, p, None, out, half)
+    if not x.is_cuda:
+        y = _adapted_cpu(x, w_gate_up, pool, p, None)
+        y = (glu_act(y[:, :half], act) * y[:, half:]).to(x.dtype)
+        return y if out is None else out.copy_(y)
+    if out is None:
+        out = torch.empty(x.shape[0], half, dtype=x.dtype, device=x.device)
+    return _run(x, w_gate_up, pool, p, None, out, GLU_ACTS[act])

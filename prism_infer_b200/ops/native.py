@@ -77,6 +77,10 @@ _SIGNATURES = {
     "prism_flash_attention": "plplppplppppppiiiiiiiiiifpi",
     "prism_kv_page_copy": "ppllippllpppiiiip",
     "prism_kv_compact": "pliplppppiiiip",
+    "prism_step_maps": "pppppp" "iiiii" "ppppppppp" "pi",
+    "prism_adapter_plan": "piiippppi",
+    "prism_adapter_shrink": "ippppp" "iiiilpi",
+    "prism_adapter_expand": "ipppppp" "iiiiipilpi",
     "prism_sample": "pllipppiilupppipi",
     "prism_merge_candidates": "pppiipi",
     "prism_lm_head_fp8_plan": "p",
@@ -111,7 +115,7 @@ _SIGNATURES = {
     "prism_decode_layers_seq_step": "i",
 }
 _STATUS_UNITS = ("gemm", "norm", "attn", "attn_tc", "kvops", "sampler", "comm", "decode_layers", "lm_head_fp8",
-                 "latent", "stream", "gemm_f32", "window", "moe", "recurrence")
+                 "latent", "stream", "gemm_f32", "window", "moe", "recurrence", "batch", "adapters")
 
 
 class NativeError(RuntimeError):

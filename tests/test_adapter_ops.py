@@ -1,0 +1,299 @@
+"""Projections with low-rank adapters against the plain statement in 64 bits.  CPU statements, and the kernels on a B200."""
+
+import os
+import sys
+
+import pytest
+import torch
+
+sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
+from op_helpers import CPU, GPU16, GPU32, rand  # noqa: E402
+
+from prism_infer_b200.ops import adapters, native  # noqa: E402
+
+BACKENDS = [CPU, GPU32, GPU16]
+GPU = [GPU32, GPU16]
+
+
+class Problem:
+    """Operands that every type holds exactly, kept on the CPU, and the pool, weights and plan on a backend."""
+
+    def __init__(self, backend, T, K, sections, rank, slots, who, seed=0, bias=False, scale=1.0):
+        device, dtype = backend
+        self.device, self.dtype, self.sections = device, dtype, sections
+        n = len(sections)
+        self.x = rand(T, K, seed=seed, scale=scale)
+        self.w = rand(sum(sections), K, seed=seed + 1, scale=K ** -0.5)
+        self.a = rand(slots, n, rank, K, seed=seed + 2, scale=K ** -0.5)
+        self.b = [rand(slots, m, rank, seed=seed + 3 + i, scale=0.5 * rank ** -0.5) for i, m in enumerate(sections)]
+        self.scale = [(1.0, 2.0, 0.5)[s % 3] for s in range(slots)]
+        self.bias = rand(sum(sections), seed=seed + 20) if bias else None
+        self.who = torch.as_tensor(who, dtype=torch.int32)
+        self.pool = adapters.AdapterPool(slots, rank, K, sections, device=device, dtype=dtype)
+        for s in range(slots):
+            self.pool.load(s, list(self.a[s]), [b[s] for b in self.b], self.scale[s])
+        self.plan = adapters.plan(self.who.to(device), slots)
+
+    def to(self, t):
+        return None if t is None else t.to(self.device, self.dtype)
+
+    def run(self, **kw):
+        return adapters.linear(self.to(self.x), self.to(self.w), self.pool, self.plan, bias=self.to(self.bias), **kw)
+
+    def exact(self):
+        """(value, bound on the error of sums in 32 bits with the low-rank products rounded to the type), both [T, M] in 64 bits.
+
+        A sum of n products in 32 bits, in any order and truncated at each step, is off by at most n 2^-23 of the sum of their
+        magnitudes; a bf16 operand is off by 2^-8 of its value, and so is the result."""
+        x, w, u = self.x.double(), self.w.double(), 2.0 ** -8 if self.dtype == torch.bfloat16 else 2.0 ** -23
+        K, f = x.shape[1], 2.0 ** -23
+        y, err = x @ w.T, (K + 8) * f * (x.abs() @ w.abs().T)
+        first = 0
+        for i, m in enumerate(self.sections):
+            for t, s in enumerate(self.who.tolist()):
+                if s < 0:
+                    continue
+                a, b = self.a[s, i].double(), self.b[i][s].double()
+                low, low_abs = self.scale[s] * (a @ x[t]), self.scale[s] * (a.abs() @ x[t].abs())
+                y[t, first:first + m] += b @ low
+                err[t, first:first + m] += b.abs() @ (u * low.abs() + (K + len(low) + 16) * f * low_abs) * 1.01
+            first += m
+        if self.bias is not None:
+            y += self.bias.double()
+        err += 8 * f * y.abs()
+        return y, err
+
+    def check(self, got, y=None, err=None):
+        if y is None:
+            y, err = self.exact()
+        last = 2.0 ** -8 if self.dtype == torch.bfloat16 else 2.0 ** -24
+        assert got.dtype == self.dtype and got.shape == y.shape
+        off = (got.double().cpu() - y).abs() - (err * 1.01 + last * (y.abs() + err) + 1e-30)
+        assert float(off.max()) <= 0, (float(off.max()), (off > 0).nonzero()[:5].tolist())
+
+
+def mixed(T, slots, seed=1, bare=0.2):
+    g = torch.Generator().manual_seed(seed)
+    who = torch.randint(0, slots, (T,), generator=g, dtype=torch.int32)
+    return torch.where(torch.rand(T, generator=g) < bare, -1, who)
+
+
+@pytest.mark.parametrize("backend", BACKENDS)
+@pytest.mark.parametrize("T", [1, 2, 15, 16, 17, 33, 64, 65, 127, 128, 129, 200, 256, 257, 300, 513])
+@pytest.mark.parametrize("K,sections,rank,slots", [(64, (128,), 16, 4), (200, (96, 40, 24), 5, 9), (8, (1,), 1, 1), (1000, (272, 16), 33, 3)])
+def test_tokens_with_adapters_in_any_order(backend, T, K, sections, rank, slots):
+    p = Problem(backend, T, K, sections, rank, slots, mixed(T, slots), bias=T % 2 == 0)
+    p.check(p.run())
+
+
+@pytest.mark.parametrize("backend", BACKENDS)
+@pytest.mark.parametrize("T,K,sections,rank,slots", [
+    (128, 320, (256,), 16, 128),            # every token an adapter of its own
+    (256, 128, (144,), 16, 256),            # and a whole tile of them
+    (400, 264, (64, 64), 64, 300),          # more slots than a tile has tokens
+    (130, 4096, (512,), 64, 2),             # a long sum
+    (40, 2048, (1024, 256, 256), 24, 20),
+])
+def test_many_adapters(backend, T, K, sections, rank, slots):
+    order = torch.randperm(slots, generator=torch.Generator().manual_seed(3)).int()
+    p = Problem(backend, T, K, sections, rank, slots, order.repeat(-(-T // slots))[:T])
+    p.check(p.run())
+
+
+@pytest.mark.parametrize("backend", BACKENDS)
+@pytest.mark.parametrize("T", [1, 40, 300])
+def test_steps_without_adapters(backend, T):
+    """Nobody has one; loaded and empty slots beside each other; slots cleared again."""
+    p = Problem(backend, T, 96, (48, 32), 8, 5, [-1] * T, bias=True)
+    plain = p.run()
+    p.check(plain)
+    p.pool.clear(3)
+    p.plan = adapters.plan(torch.full((T,), 3, dtype=torch.int32, device=p.device), 5)
+    assert torch.equal(p.run(), plain)
+
+
+@pytest.mark.parametrize("backend", BACKENDS)
+def test_ranks_and_reloading(backend):
+    """A slot loaded with a smaller rank than before keeps nothing of the one before."""
+    p = Problem(backend, 20, 64, (32, 32), 20, 2, mixed(20, 2))
+    p.run()
+    p.a, p.b = p.a[:, :, :3], [b[:, :, :3] for b in p.b]
+    for s in range(2):
+        p.pool.load(s, list(p.a[s]), [b[s] for b in p.b], p.scale[s])
+    p.check(p.run())
+
+
+@pytest.mark.parametrize("backend", BACKENDS)
+@pytest.mark.parametrize("act", ["silu", "gelu_tanh"])
+@pytest.mark.parametrize("T,K,half,rank,slots", [(1, 64, 64, 16, 2), (7, 200, 40, 5, 3), (128, 136, 96, 16, 128), (130, 64, 80, 40, 7), (300, 512, 256, 16, 5),
+                                                 (33, 72, 13, 4, 2), (300, 72, 13, 4, 2)])
+def test_gated_unit(backend, act, T, K, half, rank, slots):
+    p = Problem(backend, T, K, (half, half), rank, slots, mixed(T, slots))
+    got = adapters.gate_up_glu(p.to(p.x), p.to(p.w), p.pool, p.plan, act)
+    y, err = p.exact()
+    g, u, eg, eu = y[:, :half], y[:, half:], err[:, :half], err[:, half:]
+    unit = torch.nn.functional.silu(g) if act == "silu" else torch.nn.functional.gelu(g, approximate="tanh")
+    # both activations have slopes of at most 1.13; in bf16 their exponentials and hyperbolic tangent are approximate: 2^-10 of the unit's scale
+    fast = 2.0 ** -10 if p.dtype == torch.bfloat16 else 2.0 ** -10 if act == "gelu_tanh" and p.device != "cpu" else 2.0 ** -20
+    bound = 1.13 * eg * (u.abs() + eu) + (unit.abs() + 1.13 * eg) * eu + fast * (g.abs() + eg) * (u.abs() + eu)
+    p.check(got, unit * u, bound)
+
+
+@pytest.mark.parametrize("backend", GPU)
+def test_strided_operands_and_output(backend):
+    """Rows of a wider buffer; columns beside the output stay as they were."""
+    for T in (9, 200):
+        p = Problem(backend, T, 64, (48,), 8, 3, mixed(T, 3), bias=True)
+        x = torch.full((T, 96), 7.0, dtype=p.dtype, device=p.device)
+        x[:, 16:80] = p.to(p.x)
+        w = torch.full((48, 128), 7.0, dtype=p.dtype, device=p.device)
+        w[:, 64:] = p.to(p.w)
+        for left, width in ((8, 64), (3, 53)):
+            out = torch.full((T + 2, width), 5.0, dtype=p.dtype, device=p.device)
+            got = adapters.linear(x[:, 16:80], w[:, 64:], p.pool, p.plan, bias=p.to(p.bias), out=out[1:T + 1, left:left + 48])
+            p.check(got)
+            out[1:T + 1, left:left + 48] = 5.0
+            assert bool((out == 5.0).all())
+
+
+@pytest.mark.parametrize("backend", GPU)
+@pytest.mark.parametrize("T", [6, 300])
+def test_rows_do_not_meet(backend, T):
+    """A row that is infinite or not a number leaves the other rows as they are."""
+    p = Problem(backend, T, 128, (64,), 16, 4, mixed(T, 4, bare=0.3))
+    clean = p.run().clone()
+    bad = torch.tensor([1, T // 2])
+    p.x[bad[0], 3], p.x[bad[1]] = float("inf"), float("nan")
+    got = p.run()
+    keep = torch.ones(T, dtype=torch.bool)
+    keep[bad] = False
+    assert torch.equal(got[keep.to(got.device)], clean[keep.to(got.device)])
+    assert not bool(torch.isfinite(got[bad.to(got.device)]).any())
+
+
+@pytest.mark.parametrize("backend", GPU)
+@pytest.mark.parametrize("T", [5, 128, 300])
+def test_repeated_calls_and_graph_replays_agree(backend, T):
+    """Bit for bit, on another stream too; a replay reads new activations, adapters and plans."""
+    p = Problem(backend, T, 256, (96, 32), 16, 6, mixed(T, 6))
+    want = p.run().clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        again = p.run()
+    side.synchronize()
+    assert torch.equal(again, want)
+    x, w, who = p.to(p.x), p.to(p.w), p.who.to(p.device)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        plan = adapters.plan(who, 6)
+        y = adapters.linear(x, w, p.pool, plan)
+    graph.replay()
+    assert torch.equal(y, want)
+    q = Problem(backend, T, 256, (96, 32), 16, 6, mixed(T, 6, seed=5), seed=40)
+    x.copy_(q.to(q.x)), w.copy_(q.to(q.w)), who.copy_(q.who)
+    for s in range(6):
+        p.pool.load(s, list(q.a[s]), [b[s] for b in q.b], q.scale[s])
+    graph.replay()
+    q.check(y)
+    native.check_status()
+
+
+@pytest.mark.parametrize("backend", GPU)
+def test_calls_on_two_streams_at_once(backend):
+    a, b = (Problem(backend, T, 512, (256,), 16, 8, mixed(T, 8), seed=T) for T in (64, 300))
+    want = a.run().clone(), b.run().clone()
+    torch.cuda.synchronize()
+    streams = torch.cuda.Stream(), torch.cuda.Stream()
+    got = [], []
+    for _ in range(10):
+        for i, p in enumerate((a, b)):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(p.run())
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(g, want[i]) for g in got[i])
+
+
+def plan_of(who, slots):
+    index, lists, counts = [], [], []
+    for lo in range(0, len(who), 256):
+        here = sorted({w for w in who[lo:lo + 256] if w >= 0})
+        index += [here.index(w) if w >= 0 else -1 for w in who[lo:lo + 256]]
+        lists.append(here + [-1] * (min(slots, 256, len(who)) - len(here)))
+        counts.append(len(here))
+    return index, lists, counts
+
+
+@pytest.mark.parametrize("backend", [CPU, GPU32])
+@pytest.mark.parametrize("T", [1, 31, 256, 257, 1000])
+@pytest.mark.parametrize("slots", [1, 2, 32, 33, 300, 8192])
+def test_plan(backend, T, slots):
+    for bare in (0.0, 0.3, 1.0):
+        who = mixed(T, slots, seed=T + slots, bare=bare)
+        p = adapters.plan(who.to(backend[0]), slots)
+        assert (p.index.tolist(), p.lists.tolist(), p.counts.tolist()) == plan_of(who.tolist(), slots)
+
+
+@pytest.mark.parametrize("backend", BACKENDS)
+def test_no_tokens(backend):
+    p = Problem(backend, 0, 64, (32, 32), 8, 2, [])
+    assert p.run().shape == (0, 64)
+    assert adapters.gate_up_glu(p.to(p.x), p.to(p.w), p.pool, p.plan, "silu").shape == (0, 32)
+
+
+@pytest.mark.gpu
+def test_slots_out_of_range_count_as_none_and_are_reported():
+    p = Problem(("cuda:0", torch.bfloat16), 10, 64, (32,), 8, 2, [0, 1] * 5)
+    native.read_status()
+    plan = adapters.plan(torch.tensor([0, 1, 2, -7, 2 ** 31 - 1, 1, 0, 1, 0, 1], dtype=torch.int32, device="cuda"), 2)
+    assert plan.index.tolist() == [0, 1, -1, -1, -1, 1, 0, 1, 0, 1]
+    assert native.read_status()["adapters"][0] == 3
+    p.plan, p.who[2:5] = plan, -1
+    p.check(p.run())
+
+
+@pytest.mark.parametrize("backend", BACKENDS)
+def test_refusals(backend):
+    device, dtype = backend
+    p = Problem(backend, 4, 64, (32, 32), 8, 2, [0, 1, -1, 0])
+    x, w = p.to(p.x), p.to(p.w)
+
+    def refused(call, *args, **kw):
+        with pytest.raises(ValueError):
+            call(*args, **kw)
+
+    refused(adapters.linear, x[:, :32], w, p.pool, p.plan)
+    refused(adapters.linear, x[:3], w, p.pool, p.plan)
+    refused(adapters.linear, x, w[:32], p.pool, p.plan)
+    refused(adapters.linear, x.double(), w, p.pool, p.plan)
+    refused(adapters.linear, x.t().contiguous().t(), w, p.pool, p.plan)
+    refused(adapters.linear, x, w, p.pool, p.plan, bias=w[0, :32])
+    refused(adapters.linear, x, w, p.pool, p.plan, out=torch.empty(4, 63, dtype=dtype, device=device))
+    refused(adapters.linear, x, w, p.pool, adapters.plan(p.who.to(device), 3))
+    refused(adapters.linear, x[:1].expand(4, 64), w, p.pool, p.plan)
+    if dtype == torch.bfloat16:
+        refused(adapters.linear, torch.zeros(4 * 64 + 8, dtype=dtype, device=device)[1:257].view(4, 64), w, p.pool, p.plan)
+        refused(adapters.AdapterPool, 2, 8, 60, 32, device=device)
+    refused(adapters.gate_up_glu, x, w, p.pool, p.plan, "relu")
+    refused(adapters.gate_up_glu, x, w, adapters.AdapterPool(2, 8, 64, (16, 48), device=device, dtype=dtype), p.plan, "silu")
+    refused(adapters.plan, p.who.long().to(device), 2)
+    refused(adapters.plan, p.who.to(device), 0)
+    refused(adapters.plan, p.who.to(device), 8193)
+    refused(adapters.AdapterPool, 0, 8, 64, 32, device=device)
+    refused(adapters.AdapterPool, 2, 257, 64, 32, device=device)
+    refused(adapters.AdapterPool, 2, 8, 64, (), device=device)
+    refused(adapters.AdapterPool, 2, 8, 64, 32, device=device, dtype=torch.float16)
+    pool = adapters.AdapterPool(2, 8, 64, 32, device=device, dtype=dtype)
+    a, b = torch.ones(8, 64), torch.ones(32, 8)
+    refused(pool.load, 2, a, b)
+    refused(pool.load, 0, a, b[:, :7])
+    refused(pool.load, 0, a, b[:31])
+    refused(pool.load, 0, [a, a], [b, b])
+    refused(pool.load, 0, torch.ones(9, 64), torch.ones(32, 9))
+    refused(pool.load, 0, a, b, float("nan"))
+    refused(pool.load, 0, a, b * float("inf"))
+    refused(pool.load, 0, a * 1e39, b)
+    refused(pool.clear, -1)
+    if device == "cpu":
+        refused(adapters.plan, torch.tensor([2], dtype=torch.int32), 2)
