@@ -175,21 +175,42 @@ def _adapted_cpu(x, w, pool, p, bias):
     return y
 
 
+# bytes of low-rank rows in one launch; a step that needs more runs in runs of tokens
+MAX_LOW_BYTES = 256 << 20
+
+
 def _run(x, w, pool, p, bias, out, act):
-    T, f32 = x.shape[0], int(pool.dtype == torch.float32)
+    T = x.shape[0]
     if T == 0:
         return out
+    if pool.dtype == torch.float32:
+        return _run_f32(x, w, pool, p, bias, out, act)
+    capacity, all_panels = p.lists.shape[1], pool.low // PANEL
+    tile_rows = TILE_TOKENS if T > 128 else max(16, 1 << (T - 1).bit_length())
+    per_tile = capacity * all_panels * tile_rows * PANEL     # values of every panel that a tile's adapters may need
+    tiles = p.lists.shape[0]
+    run = min(tiles, max(1, MAX_LOW_BYTES // (2 * per_tile)))
+    h = torch.empty(run * per_tile, dtype=torch.bfloat16, device=x.device)
+    for first in range(0, tiles, run):
+        t0, n = first * TILE_TOKENS, min(run * TILE_TOKENS, T - first * TILE_TOKENS)
+        if tiles > run:
+            tile_rows = TILE_TOKENS if n > 128 else max(16, 1 << (n - 1).bit_length())
+        native.call("prism_adapter_linear", x.data_ptr() + 2 * t0 * _ld(x), _p(w), _p(pool.a), _p(pool.b), _p(pool.scale), p.index.data_ptr() + 4 * t0,
+                    p.lists.data_ptr() + 4 * first * capacity, p.counts.data_ptr() + 4 * first, _p(bias), out.data_ptr() + 2 * t0 * _ld(out), _p(h), n,
+                    pool.features, pool.in_features, pool.slots, pool.panels, len(pool.sections), pool._ends, capacity, tile_rows, act, _ld(x), _ld(w),
+                    _ld(out), _s(), _pdl())
+    return out
+
+
+def _run_f32(x, w, pool, p, bias, out, act):
+    T = x.shape[0]
     base = torch.empty(T, pool.features, dtype=torch.float32, device=x.device)
-    if f32:
-        native.call("prism_gemm_f32", _p(w), _p(x), _p(base), pool.features, T, pool.in_features, _ld(w), _ld(x), pool.features,
-                    None, 0, None, None, None, 0.0, _s(), _pdl())
-    else:
-        native.call("prism_gemm_wx", _p(w), _p(x), _p(base), pool.features, T, pool.in_features, _ld(w), _ld(x), pool.features,
-                    pool.features, None, None, 0, 0, 0, 0, 1, 1, 0, 0, 0, _s(), _pdl())
+    native.call("prism_gemm_f32", _p(w), _p(x), _p(base), pool.features, T, pool.in_features, _ld(w), _ld(x), pool.features,
+                None, 0, None, None, None, 0.0, _s(), _pdl())
     h = torch.empty(T, pool.low, dtype=torch.float32, device=x.device)
-    native.call("prism_adapter_shrink", f32, _p(x), _p(pool.a), _p(pool.scale), _p(p.adapter), _p(h), T, pool.in_features, pool.low, pool.slots,
+    native.call("prism_adapter_shrink", 1, _p(x), _p(pool.a), _p(pool.scale), _p(p.adapter), _p(h), T, pool.in_features, pool.low, pool.slots,
                 _ld(x), _s(), _pdl())
-    native.call("prism_adapter_expand", f32, _p(base), _p(h), _p(pool.b), _p(bias), _p(p.adapter), _p(out), T, pool.features, pool.panels,
+    native.call("prism_adapter_expand", 1, _p(base), _p(h), _p(pool.b), _p(bias), _p(p.adapter), _p(out), T, pool.features, pool.panels,
                 pool.slots, len(pool.sections), pool._ends, act, _ld(out), _s(), _pdl())
     return out
 

@@ -6,6 +6,7 @@
 // section after section; B as [slot][panel of a section][feature][16], so that the 16 ranks of a run of features are one piece of memory.
 #include "common.cuh"
 
+#include <atomic>
 #include <type_traits>
 
 PRISM_DEFINE_TU_STATUS(adapters)
@@ -140,6 +141,507 @@ __global__ void __launch_bounds__(256) adapter_expand_kernel(const ExpandArgs a)
   else *out = __float2bfloat16_rn(v);
 }
 
+// ------------------------------------------------------------------------------------------------------------------------------------
+// bf16 on the tensor cores: two launches, the low-rank rows (adapter_low_kernel) and the projection with them (adapter_gemm_kernel, or
+// gemm_pair.cuh from 129 tokens).
+//
+// Tokens of different adapters share tiles.  A tile's adapters (AdapterPlan.lists) become panels of 16 ranks: in the first kernel 128
+// rows of A of up to eight panels multiply all tokens of the tile, and what is kept is each token's row in its own adapter's panels,
+// zeros elsewhere; in the second every panel is one more MMA of 16 columns in the sum of the projection.  Both waste tensor cycles on
+// tokens of other adapters, which a weight stream (decode) hides and a sum over K dwarfs (prompts), and both read every factor once.
+// The low-rank row is rounded to bf16, as an operand of the matrix instructions has to be; scale and sums are 32-bit.
+// ------------------------------------------------------------------------------------------------------------------------------------
+constexpr int TC_THREADS = 192;         // TMA warp, MMA warp, four epilogue warps
+constexpr int W_BYTES = 128 * 64 * 2;   // 128 rows of a k-block of 64
+constexpr int RED_PITCH = 132;          // floats of one token's 128 sums in shared memory
+
+template <int BN>
+__host__ __device__ constexpr int stage_bytes() { return W_BYTES + BN * 128; }
+
+__device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ float4 add4(const float4& a, const float4& b) { return make_float4(a.x + b.x, a.y + b.y, a.z + b.z, a.w + b.w); }
+__device__ __forceinline__ uint2 pack4(const float4& v) {
+  uint2 o;
+  *reinterpret_cast<__nv_bfloat162*>(&o.x) = __floats2bfloat162_rn(v.x, v.y);
+  *reinterpret_cast<__nv_bfloat162*>(&o.y) = __floats2bfloat162_rn(v.z, v.w);
+  return o;
+}
+// Share z of a sum over kb k-blocks in CS parts, none of them empty (CS <= kb).
+__device__ __forceinline__ int part_begin(int kb, int z, int cs) { return (int)((long long)kb * z / cs); }
+
+// One token's 128 sums of the accumulator (lane = row) to shared memory, token after token.
+template <int BN>
+__device__ __forceinline__ void accumulator_to_smem(uint32_t tmem, float* red, int q, int lane, int tokens) {
+  const uint32_t t_lane = tmem + ((uint32_t)(q * 32) << 16);
+  for (int c0 = 0; c0 < tokens; c0 += 16) {
+    uint32_t r[16];
+    tmem_ld16(t_lane + c0, r);
+    tmem_ld_wait();
+#pragma unroll
+    for (int j = 0; j < 16; ++j) red[(c0 + j) * RED_PITCH + q * 32 + lane] = __uint_as_float(r[j]);
+  }
+}
+
+struct LowArgs {
+  const int* lists;      // [tiles][capacity]
+  const int* counts;     // [tiles]
+  const int* index;      // [T]
+  const float* scale;    // [slots]
+  bf16* h;               // [tiles][capacity][all_panels][tile_rows][16]
+  int T, kb, capacity, all_panels, tile_rows, stages;
+};
+
+// h of one tile of BN tokens: cluster (1, 1, CS) splits K, its CTAs add their sums through one another's shared memory.
+template <int BN>
+__global__ void __launch_bounds__(TC_THREADS, 1)
+adapter_low_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmX, const LowArgs a) {
+  constexpr int TMEM_COLS = BN < 32 ? 32 : BN, STAGE = stage_bytes<BN>();
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  float* const red = reinterpret_cast<float*>(smem);   // the ring's memory, between two groups of panels
+  const int stages = a.stages;
+  const size_t ring = max((size_t)stages * STAGE, (size_t)BN * RED_PITCH * 4);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + ring);
+  uint64_t* empty = full + stages;
+  uint64_t* acc_full = empty + stages;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 1);
+  const int warp = uniform_warp(), lane = threadIdx.x & 31;
+  const int cs = gridDim.z, z = blockIdx.z, token0 = blockIdx.y * BN, tile = token0 / PLAN_TILE;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < stages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    mbar_init(acc_full, 1);
+    fence_barrier_init();
+    tma_prefetch_desc(&tmA);
+    tma_prefetch_desc(&tmX);
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, TMEM_COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  pdl_launch_dependents();
+  pdl_wait();   // tokens and plan come from the previous kernels, and h may still be read by them
+
+  const int panels = min(a.counts[tile], a.capacity) * a.all_panels;
+  const int* const list = a.lists + (size_t)tile * a.capacity;
+  const int kb0 = part_begin(a.kb, z, cs), kb1 = part_begin(a.kb, z + 1, cs);
+  int s = 0, round = 0;   // ring stage; groups of panels done
+  uint32_t parity = 0;    // of the full barriers (MMA); the producer waits for the phase before
+  bool ok = true;         // this thread's role goes on; after a wait that ran out it only keeps step with the cluster
+  for (int p0 = blockIdx.x * 8; p0 < panels; p0 += gridDim.x * 8, ++round) {
+    const int np = min(8, panels - p0);
+    if (warp == 0) {
+      if (elect_one() && ok) {
+        int row[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int p = p0 + min(i, np - 1), j = p / a.all_panels;
+          row[i] = (list[j] * a.all_panels + (p - j * a.all_panels)) * 16;
+        }
+        for (int kb = kb0; kb < kb1; ++kb) {
+          ok = mbar_wait(&empty[s], parity ^ 1, 1);
+          if (!ok) break;
+          uint8_t* const st = smem + (size_t)s * STAGE;
+          mbar_expect_tx(&full[s], np * 2048 + BN * 128);
+          tma_load_2d(st + W_BYTES, &tmX, &full[s], kb * 64, token0);
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (i < np) tma_load_2d(st + i * 2048, &tmA, &full[s], kb * 64, row[i]);
+          if (++s == stages) s = 0, parity ^= 1;
+        }
+        if (!ok) {
+          // unwinding: copies already in flight land before shared memory is used for the sums
+          for (int j = 0; j < stages; ++j) {
+            if (--s < 0) s = stages - 1, parity ^= 1;
+            (void)mbar_wait(&full[s], parity, 4);
+          }
+        }
+      }
+    } else if (warp == 1) {
+      if (elect_one() && ok) {
+        constexpr uint32_t idesc = umma_idesc_bf16(128, BN);
+        for (int kb = kb0; kb < kb1; ++kb) {
+          ok = mbar_wait(&full[s], parity, 2);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t st = smem_u32(smem + (size_t)s * STAGE);
+          const uint64_t da = umma_desc_sw128(st), db = umma_desc_sw128(st + W_BYTES);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) tc_mma_f16(tmem, da + 2 * k, db + 2 * k, idesc, kb != kb0 || k != 0);
+          tc_commit(&empty[s]);
+          if (++s == stages) s = 0, parity ^= 1;
+        }
+        if (ok) tc_commit(acc_full);
+      }
+    } else {
+      // rows of unused panels hold what earlier loads left; nothing reads them
+      ok = ok && __all_sync(0xffffffffu, mbar_wait(acc_full, round & 1, 3));
+      if (ok) {
+        tc_fence_after();
+        accumulator_to_smem<BN>(tmem, red, warp & 3, lane, BN);
+      }
+    }
+    tc_fence_before();
+    __syncwarp();
+    cluster_sync_all();
+    tc_fence_after();
+    // items of four ranks: the ranks of a token's panel fastest, then its tokens; every CTA takes its share of the tokens
+    const int share = BN / cs, first = z * share;
+    for (int i = threadIdx.x; i < np * share * 4; i += TC_THREADS) {
+      const int quarter = i & 3, c = first + (i >> 2) % share, g = (i >> 2) / share, p = p0 + g, j = p / a.all_panels, t = token0 + c;
+      float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (t < a.T && a.index[t] == j) {
+        for (int peer = 0; peer < cs; ++peer) v = add4(v, ld_cluster4(cluster_addr(red + c * RED_PITCH + g * 16 + quarter * 4, peer)));
+        const float scale = a.scale[list[j]];
+        v = make_float4(v.x * scale, v.y * scale, v.z * scale, v.w * scale);
+      }
+      const size_t at = (((size_t)tile * a.capacity * a.all_panels + p) * a.tile_rows + (t - tile * PLAN_TILE)) * 16 + quarter * 4;
+      *reinterpret_cast<uint2*>(a.h + at) = pack4(v);
+    }
+    // the ring is written again by copies once every CTA has read the sums
+    fence_proxy_async();
+    cluster_sync_all();
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, TMEM_COLS);
+  }
+}
+
+struct TileArgs {
+  const int* lists;
+  const int* counts;
+  const bf16* bias;      // [M] (null: none)
+  bf16* out;             // [T][ldo]
+  long long ldo;
+  int T, M, kb, capacity, panels, all_panels, tile_rows, stages;
+  int act;               // DUAL: PRISM_GLU_*
+  int no_row;            // a row behind all of B, which reads as zeros
+  int vec;               // four features of a row can be stored at once
+  int sections;
+  int start[MAX_SECTIONS], end[MAX_SECTIONS], first_tile[MAX_SECTIONS];
+};
+
+// 128 features (DUAL: 64 gates and their 64 ups) of BN tokens.  Weights are the A operand and stream once; cluster (1, 1, CS) splits the
+// k-blocks and the panels of the tile's adapters, and adds the parts through shared memory.
+template <int BN, bool DUAL>
+__global__ void __launch_bounds__(TC_THREADS, 1)
+adapter_gemm_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmB,
+                    const __grid_constant__ CUtensorMap tmH, const TileArgs a) {
+  constexpr int TMEM_COLS = BN < 32 ? 32 : BN, STAGE = stage_bytes<BN>(), FEATURES = DUAL ? 64 : 128;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  float* const red = reinterpret_cast<float*>(smem);   // the ring's memory, once the sums are done
+  const int stages = a.stages;
+  const size_t ring = max((size_t)stages * STAGE, (size_t)BN * RED_PITCH * 4);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + ring);
+  uint64_t* empty = full + stages;
+  uint64_t* acc_full = empty + stages;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 1);
+  const int warp = uniform_warp(), lane = threadIdx.x & 31;
+  const int cs = gridDim.z, z = blockIdx.z, token0 = blockIdx.y * BN, tile = token0 / PLAN_TILE;
+  int section = 0;
+  if (!DUAL)
+    while (section + 1 < a.sections && (int)blockIdx.x >= a.first_tile[section + 1]) ++section;
+  const int f0 = DUAL ? blockIdx.x * FEATURES : a.start[section] + ((int)blockIdx.x - a.first_tile[section]) * FEATURES;
+  const int f_end = DUAL ? a.M / 2 : a.end[section];
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < stages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    mbar_init(acc_full, 1);
+    fence_barrier_init();
+    tma_prefetch_desc(&tmW);
+    tma_prefetch_desc(&tmX);
+    tma_prefetch_desc(&tmB);
+    tma_prefetch_desc(&tmH);
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, TMEM_COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  pdl_launch_dependents();
+
+  const int kb0 = part_begin(a.kb, z, cs), kb1 = part_begin(a.kb, z + 1, cs);
+  const int per = DUAL ? a.all_panels : a.panels;   // panels of one adapter that reach this tile
+  if (warp == 0) {
+    if (elect_one()) {
+      auto load_w = [&](int s, int kb) {
+        uint8_t* const st = smem + (size_t)s * STAGE;
+        mbar_expect_tx(&full[s], STAGE);
+        tma_load_2d(st, &tmW, &full[s], kb * 64, f0);
+        if (DUAL) tma_load_2d(st + W_BYTES / 2, &tmW, &full[s], kb * 64, a.M / 2 + f0);
+      };
+      const int pre = min(stages, kb1 - kb0);
+      for (int i = 0; i < pre; ++i) load_w(i, kb0 + i);   // weights depend on no earlier kernel
+      pdl_wait();
+      const int extra = min(a.counts[tile], a.capacity) * per;
+      const int* const list = a.lists + (size_t)tile * a.capacity;
+      int s = 0;
+      uint32_t parity = 1;   // a fresh empty barrier counts as free
+      bool ok = true;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        ok = mbar_wait(&empty[s], parity, 1);
+        if (!ok) break;
+        if (kb - kb0 >= pre) load_w(s, kb);
+        tma_load_2d(smem + (size_t)s * STAGE + W_BYTES, &tmX, &full[s], kb * 64, token0);
+        if (++s == stages) s = 0, parity ^= 1;
+      }
+      for (int e0 = z * 4; e0 < extra && ok; e0 += cs * 4) {
+        const int n = min(4, extra - e0);
+        int slot[4];   // asked for before the wait
+#pragma unroll
+        for (int i = 0; i < 4; ++i) slot[i] = i < n ? list[(e0 + i) / per] : 0;
+        ok = mbar_wait(&empty[s], parity, 1);
+        if (!ok) break;
+        uint8_t* const st = smem + (size_t)s * STAGE;
+        mbar_expect_tx(&full[s], n * (4096 + BN * 32));
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (i < n) {
+            const int j = (e0 + i) / per, q = (e0 + i) - j * per, of = DUAL ? q : section * a.panels + q;
+            const int row = (slot[i] * a.panels + of % a.panels) * a.M;
+            if (DUAL) {   // a gate's panel adds nothing to the up half, and the other way round
+              const bool up = of >= a.panels;
+              tma_load_2d(st + i * 4096, &tmB, &full[s], 0, up ? a.no_row : row + f0);
+              tma_load_2d(st + i * 4096 + 2048, &tmB, &full[s], 0, up ? row + a.M / 2 + f0 : a.no_row);
+            } else {
+              tma_load_2d(st + i * 4096, &tmB, &full[s], 0, row + f0);
+            }
+            tma_load_2d(st + W_BYTES + i * BN * 32, &tmH, &full[s], 0,
+                        ((tile * a.capacity + j) * a.all_panels + of) * a.tile_rows + (token0 - tile * PLAN_TILE));
+          }
+        if (++s == stages) s = 0, parity ^= 1;
+      }
+      if (!ok) {
+        // unwinding after a timed-out wait: copies already in flight land before shared memory is used for the sums
+        for (int j = 0; j < stages; ++j) {
+          if (--s < 0) s = stages - 1, parity ^= 1;
+          (void)mbar_wait(&full[s], parity ^ 1, 4);
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (elect_one()) {
+      constexpr uint32_t idesc = umma_idesc_bf16(128, BN);
+      pdl_wait();   // the number of panels comes from the previous kernels
+      const int extra = min(a.counts[tile], a.capacity) * per;
+      int s = 0;
+      uint32_t parity = 0;
+      bool ok = true;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        ok = mbar_wait(&full[s], parity, 2);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t st = smem_u32(smem + (size_t)s * STAGE);
+        const uint64_t da = umma_desc_sw128(st), db = umma_desc_sw128(st + W_BYTES);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) tc_mma_f16(tmem, da + 2 * k, db + 2 * k, idesc, kb != kb0 || k != 0);
+        tc_commit(&empty[s]);
+        if (++s == stages) s = 0, parity ^= 1;
+      }
+      for (int e0 = z * 4; e0 < extra && ok; e0 += cs * 4) {
+        ok = mbar_wait(&full[s], parity, 2);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t st = smem_u32(smem + (size_t)s * STAGE);
+        for (int i = 0; i < min(4, extra - e0); ++i) tc_mma_f16(tmem, umma_desc_sw32(st + i * 4096), umma_desc_sw32(st + W_BYTES + i * BN * 32), idesc, 1);
+        tc_commit(&empty[s]);
+        if (++s == stages) s = 0, parity ^= 1;
+      }
+      if (ok) tc_commit(acc_full);
+    }
+  } else {
+    pdl_wait();
+    if (__all_sync(0xffffffffu, mbar_wait(acc_full, 0, 3))) {
+      tc_fence_after();
+      accumulator_to_smem<BN>(tmem, red, warp & 3, lane, min(BN, a.T - token0));
+    }
+  }
+  tc_fence_before();
+  __syncwarp();
+  cluster_sync_all();
+  // items of four features of a token, features fastest, shared out among the CTAs of the cluster
+  constexpr int QUADS = FEATURES / 4;
+  const int items = min(BN, a.T - token0) * QUADS;
+  for (int i = part_begin(items, z, cs) + threadIdx.x; i < part_begin(items, z + 1, cs); i += TC_THREADS) {
+    const int c = i / QUADS, f = f0 + (i % QUADS) * 4, n = min(4, f_end - f);
+    if (n <= 0) continue;
+    auto sum_at = [&](int row) {
+      float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      for (int peer = 0; peer < cs; ++peer) v = add4(v, ld_cluster4(cluster_addr(red + c * RED_PITCH + row, peer)));
+      return v;
+    };
+    float4 v = sum_at((i % QUADS) * 4);
+    float* const x = &v.x;
+    if (DUAL) {
+      const float4 u = sum_at(64 + (i % QUADS) * 4);
+      v = make_float4(glu(v.x, u.x, a.act), glu(v.y, u.y, a.act), glu(v.z, u.z, a.act), glu(v.w, u.w, a.act));
+    } else if (a.bias != nullptr) {
+      for (int e = 0; e < n; ++e) x[e] += __bfloat162float(a.bias[f + e]);
+    }
+    bf16* const dst = a.out + (size_t)(token0 + c) * a.ldo + f;
+    if (a.vec && n == 4) *reinterpret_cast<uint2*>(dst) = pack4(v);
+    else
+      for (int e = 0; e < n; ++e) dst[e] = __float2bfloat16_rn(x[e]);
+  }
+  // nobody leaves while a peer may read its sums
+  cluster_sync_all();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, TMEM_COLS);
+  }
+}
+
+constexpr int SMS = 148;
+constexpr int SMEM_LIMIT = 232448;   // 227 KB
+
+// Dynamic shared memory above 48 KB has to be allowed once per kernel and device.
+template <typename Kernel>
+cudaError_t allow_smem(Kernel kernel, std::atomic<unsigned long long>& devices) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const unsigned long long bit = 1ull << (dev & 63);
+  if (devices.load(std::memory_order_acquire) & bit) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_LIMIT);
+  if (e == cudaSuccess) devices.fetch_or(bit, std::memory_order_release);
+  return e;
+}
+
+// Ring stages in `budget` bytes, and the whole of the dynamic shared memory.
+template <int BN>
+int ring_stages(int budget, size_t& smem) {
+  int stages = (budget - 1024 - 256) / stage_bytes<BN>();
+  if (stages > 12) stages = 12;
+  if (stages < 2) stages = 2;
+  size_t ring = (size_t)stages * stage_bytes<BN>();
+  if (ring < (size_t)BN * RED_PITCH * 4) ring = (size_t)BN * RED_PITCH * 4;
+  smem = 1024 + ring + (2 * stages + 1) * 8 + 16;
+  return stages;
+}
+
+int power_below(int n) {   // the largest of 1, 2, 4, 8 that is not above n
+  return n >= 8 ? 8 : n >= 4 ? 4 : n >= 2 ? 2 : 1;
+}
+
+struct Call {
+  const void *x, *w;
+  long long ldx, ldw;
+  const void *a, *b;
+  const float* scale;
+  const int* index;
+  PrismAdapterTerms terms;
+  const void* bias;
+  void* out;
+  long long ldo;
+  void* h;
+  int T, M, K, act, tile_rows;
+  cudaStream_t stream;
+  bool pdl;
+};
+
+template <int BN>
+int launch_low(const Call& c) {
+  static std::atomic<unsigned long long> devices{0};
+  cudaError_t e = allow_smem(adapter_low_kernel<BN>, devices);
+  if (e != cudaSuccess) return (int)e;
+  const int all = c.terms.panels * c.terms.sec.n, tiles = (c.T + BN - 1) / BN;
+  LowArgs a{c.terms.lists, c.terms.counts, c.index, c.scale, (bf16*)c.h, c.T, (c.K + 63) / 64, c.terms.capacity, all, c.tile_rows, 0};
+  // A decode step may bring as many adapters as tokens; the tiles of a prompt hold runs of a few requests.
+  const int groups = c.T <= 128 ? (c.terms.capacity * all + 7) / 8 : 1;
+  int cs = power_below(SMS / (groups * tiles > SMS ? SMS : groups * tiles));
+  if (cs > a.kb) cs = power_below(a.kb);
+  const int gx = SMS / (tiles * cs);
+  size_t smem;
+  a.stages = ring_stages<BN>(113 * 1024, smem);
+  CUtensorMap ta, tx;
+  int rc = prism_get_tensor_map(c.a, (unsigned long long)c.terms.slots * all * 16, (unsigned long long)c.K, (unsigned long long)c.K, 16, &ta);
+  if (!rc) rc = prism_get_tensor_map(c.x, (unsigned long long)c.T, (unsigned long long)c.K, (unsigned long long)c.ldx, BN, &tx);
+  if (rc) return rc;
+  const int most = (c.terms.capacity * all + 7) / 8;
+  return (int)prism_launch_clusters(adapter_low_kernel<BN>, dim3(gx < 1 ? 1 : gx < most ? gx : most, tiles, cs), dim3(TC_THREADS), smem, c.stream,
+                                    c.pdl, cs, ta, tx, a);
+}
+
+template <int BN, bool DUAL>
+int launch_tiles(const Call& c) {
+  static std::atomic<unsigned long long> devices{0};
+  cudaError_t e = allow_smem(adapter_gemm_kernel<BN, DUAL>, devices);
+  if (e != cudaSuccess) return (int)e;
+  constexpr int FEATURES = DUAL ? 64 : 128;
+  const PrismAdapterTerms& t = c.terms;
+  const int all = t.panels * t.sec.n, token_tiles = (c.T + BN - 1) / BN;
+  TileArgs a = {};
+  a.lists = t.lists;
+  a.counts = t.counts;
+  a.bias = (const bf16*)c.bias;
+  a.out = (bf16*)c.out;
+  a.ldo = c.ldo;
+  a.T = c.T;
+  a.M = c.M;
+  a.kb = (c.K + 63) / 64;
+  a.capacity = t.capacity;
+  a.panels = t.panels;
+  a.all_panels = all;
+  a.tile_rows = c.tile_rows;
+  a.act = c.act;
+  a.no_row = t.slots * t.panels * c.M;
+  a.sections = t.sec.n;
+  a.vec = (reinterpret_cast<uintptr_t>(c.out) & 7) == 0 && c.ldo % 4 == 0;
+  int m_tiles = 0;
+  for (int s = 0; s < t.sec.n; ++s) {
+    a.start[s] = s == 0 ? 0 : t.sec.end[s - 1];
+    a.end[s] = t.sec.end[s];
+    a.first_tile[s] = m_tiles;
+    m_tiles += (a.end[s] - a.start[s] + FEATURES - 1) / FEATURES;
+    if (a.start[s] % 4) a.vec = 0;
+  }
+  if (DUAL) m_tiles = (c.M / 2 + FEATURES - 1) / FEATURES;
+  const long long tiles = (long long)m_tiles * token_tiles;
+  int cs = tiles > SMS ? 1 : power_below((int)(2 * SMS / tiles));
+  if (cs > a.kb) cs = power_below(a.kb);
+  size_t smem;
+  a.stages = ring_stages<BN>(tiles * cs <= SMS ? SMEM_LIMIT : 113 * 1024, smem);
+  CUtensorMap tw, tx, tb, th;
+  int rc = prism_get_tensor_map(c.w, (unsigned long long)c.M, (unsigned long long)c.K, (unsigned long long)c.ldw, FEATURES, &tw);
+  if (!rc) rc = prism_get_tensor_map(c.x, (unsigned long long)c.T, (unsigned long long)c.K, (unsigned long long)c.ldx, BN, &tx);
+  if (!rc) rc = prism_make_panel_tensor_map(c.b, (unsigned long long)t.slots * t.panels * c.M, FEATURES, &tb);
+  if (!rc) rc = prism_make_panel_tensor_map(c.h, (unsigned long long)t.tiles * t.capacity * all * c.tile_rows, BN, &th);
+  if (rc) return rc;
+  // the launch before is this call's own, which waited for everything older: its early loads are weights
+  return (int)prism_launch_clusters(adapter_gemm_kernel<BN, DUAL>, dim3(m_tiles, token_tiles, cs), dim3(TC_THREADS), smem, c.stream, true, cs, tw, tx, tb,
+                                    th, a);
+}
+
+template <int BN>
+int launch_both(const Call& c) {
+  const int rc = launch_low<BN>(c);
+  if (rc) return rc;
+  if (c.T > 128 && prism_adapter_pair_fits(c.M, c.act != 0, c.terms, c.out, c.ldo, c.bias))
+    return prism_adapter_pair(c.w, c.x, c.out, c.M, c.T, c.K, c.ldw, c.ldx, c.ldo, c.bias, c.act != 0, c.act, c.terms, c.stream, true);
+  return c.act ? launch_tiles<BN, true>(c) : launch_tiles<BN, false>(c);
+}
+
 }  // namespace
 
 // index [T], lists [tiles][capacity], counts [tiles], for tiles of 256 tokens.
@@ -167,4 +669,57 @@ PRISM_API int prism_adapter_expand(int f32, const void* base, const void* h, con
   const int features = gated ? M / 2 : M;
   return (int)prism_launch(f32 ? adapter_expand_kernel<float> : adapter_expand_kernel<bf16>, dim3((features + 255) / 256, T), dim3(256), 0,
                            (cudaStream_t)stream, pdl != 0, e);
+}
+
+// bf16 projection (act 0) or gated unit (PRISM_GLU_*) with the adapters of a plan.  lists, counts: of the call's tiles of 256 tokens;
+// h: tiles x capacity x all panels x tile_rows x 16 bf16 of workspace, tile_rows 16, 32, 64, 128 (as many as the tokens need) or 256.
+PRISM_API int prism_adapter_linear(const void* x, const void* w, const void* a, const void* b, const void* scale, const void* index,
+                                   const void* lists, const void* counts, const void* bias, void* out, void* h, int T, int M, int K, int slots,
+                                   int panels, int sections, const void* ends, int capacity, int tile_rows, int act, long long ldx, long long ldw,
+                                   long long ldo, void* stream, int pdl) {
+  if (T < 1 || M < 1 || K < 1 || K % 8 || slots < 1 || panels < 1 || sections < 1 || sections > MAX_SECTIONS || capacity < 1) return -1;
+  if (act && (M % 2 || sections != 2 || bias != nullptr)) return -2;
+  const int bn = T <= 16 ? 16 : T <= 32 ? 32 : T <= 64 ? 64 : 128;
+  if (tile_rows != (T <= 128 ? bn : PLAN_TILE)) return -3;
+  Call c = {};
+  c.x = x;
+  c.w = w;
+  c.ldx = ldx;
+  c.ldw = ldw;
+  c.a = a;
+  c.b = b;
+  c.scale = (const float*)scale;
+  c.index = (const int*)index;
+  c.terms.h = h;
+  c.terms.b = b;
+  c.terms.lists = (const int*)lists;
+  c.terms.counts = (const int*)counts;
+  c.terms.tiles = (T + PLAN_TILE - 1) / PLAN_TILE;
+  c.terms.capacity = capacity;
+  c.terms.panels = panels;
+  c.terms.slots = slots;
+  c.terms.sec.n = sections;
+  for (int s = 0; s < sections; ++s) {
+    c.terms.sec.end[s] = ((const int*)ends)[s];
+    if (c.terms.sec.end[s] <= (s ? c.terms.sec.end[s - 1] : 0)) return -4;
+  }
+  if (c.terms.sec.end[sections - 1] != M) return -4;
+  if ((long long)slots * panels * M >= 0x7fffffffll || (long long)c.terms.tiles * capacity * panels * sections * tile_rows >= 0x7fffffffll) return -5;
+  c.bias = bias;
+  c.out = out;
+  c.ldo = ldo;
+  c.h = h;
+  c.T = T;
+  c.M = M;
+  c.K = K;
+  c.act = act;
+  c.tile_rows = tile_rows;
+  c.stream = (cudaStream_t)stream;
+  c.pdl = pdl != 0;
+  switch (bn) {
+    case 16: return launch_both<16>(c);
+    case 32: return launch_both<32>(c);
+    case 64: return launch_both<64>(c);
+    default: return launch_both<128>(c);
+  }
 }

@@ -375,6 +375,16 @@ __device__ __forceinline__ uint64_t umma_desc_sw128(uint32_t smem_addr) {
   d |= (uint64_t)2 << 61;            // SWIZZLE_128B
   return d;
 }
+// K-major bf16 tile whose rows are 32 bytes (16 elements, one MMA's worth) with the 32-byte swizzle: 8-row groups are 256 bytes apart.
+__device__ __forceinline__ uint64_t umma_desc_sw32(uint32_t smem_addr) {
+  uint64_t d = 0;
+  d |= (uint64_t)((smem_addr & 0x3FFFFu) >> 4);
+  d |= (uint64_t)1 << 16;
+  d |= (uint64_t)(256 >> 4) << 32;
+  d |= (uint64_t)1 << 46;
+  d |= (uint64_t)6 << 61;            // SWIZZLE_32B
+  return d;
+}
 // MN-major bf16 tile with the 128-byte swizzle: rows are 64 elements along M/N (128 bytes), one
 // row per K index; 8-row groups along K are 1024 bytes apart (stride byte offset) and the next
 // 64 elements along M/N start lbo_bytes further on (leading byte offset).
@@ -402,6 +412,24 @@ int prism_get_tensor_map(const void* ptr, unsigned long long rows, unsigned long
 // head_dim read as zeros); see gemm_tcgen05.cu.
 int prism_make_head_tensor_map(const void* ptr, unsigned long long tokens, unsigned heads, unsigned head_dim,
                                unsigned long long ld, unsigned box_rows, CUtensorMap* out);
+// [rows][16] bf16 panels (contiguous rows of 32 bytes), box = box_rows x 16, 32-byte swizzle; not cached.
+int prism_make_panel_tensor_map(const void* ptr, unsigned long long rows, unsigned box_rows, CUtensorMap* out);
+// Prompt products with low-rank adapters on SM pairs (gemm_pair.cuh), as adapters.cu describes them.
+struct PrismAdapterSections {
+  int n;            // sections of the stacked matrix
+  int end[8];       // first feature behind each
+};
+struct PrismAdapterTerms {
+  const void* h;            // [tiles of 256 tokens][capacity][panels of all sections][256][16]: a token's low-rank row in its adapter's panels, else zeros
+  const void* b;            // [slots][panels][M][16]
+  const int* lists;         // [tiles][capacity] slots in use
+  const int* counts;        // [tiles]
+  int tiles, capacity, panels, slots;
+  PrismAdapterSections sec;
+};
+bool prism_adapter_pair_fits(int M, int dual, const PrismAdapterTerms& t, const void* out, long long ldo, const void* bias);
+int prism_adapter_pair(const void* W, const void* X, void* out, int M, int T, int K, long long ldw, long long ldx, long long ldo,
+                       const void* bias, int dual, int act, const PrismAdapterTerms& t, cudaStream_t stream, bool pdl);
 struct PrismLaunch {
   cudaStream_t stream;
   int pdl;  // 1: launch with programmatic stream serialization

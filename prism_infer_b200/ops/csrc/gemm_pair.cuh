@@ -122,8 +122,22 @@ __device__ __forceinline__ void add_bf16x8(float* v, const uint4& x) {
   }
 }
 
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
-gemm_pair_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW, const PairArgs a) {
+// Low-rank adapters in the same accumulators (adapters.cu has the formula and the panels).  A token tile's adapters are more k-blocks of
+// its sum: up to four panels of 16 ranks each, for which A is the tokens' low-rank rows, zero where a token has another adapter, and B
+// the panel's run of features, so neither the outputs nor the base product are touched twice.  Zeros cost tensor cycles only: an adapter
+// of rank 16 is 1/256 of a sum over 4096.
+struct PairAdapters {
+  const int* lists;
+  const int* counts;
+  int capacity, panels, all_panels;   // panels of one section, of all sections
+  int b_rows, no_row;                 // rows of one panel of B (features); a row behind all of them, which reads as zeros
+  int sections;
+  int start[8], end[8], first_tile[8];  // feature tiles do not cross sections
+};
+
+template <bool ADAPTERS>
+__device__ __forceinline__ void gemm_pair_body(const CUtensorMap& tmX, const CUtensorMap& tmW, const CUtensorMap& tmH, const CUtensorMap& tmB,
+                                               const PairArgs& a, const PairAdapters& d) {
   constexpr int A_BYTES = 128 * 64 * 2;
   constexpr int BUF_COLS = 256, TMEM_COLS = 512;
   extern __shared__ uint8_t smem_raw[];
@@ -155,6 +169,10 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant_
     fence_barrier_init();
     tma_prefetch_desc(&tmX);
     tma_prefetch_desc(&tmW);
+    if (ADAPTERS) {
+      tma_prefetch_desc(&tmH);
+      tma_prefetch_desc(&tmB);
+    }
   }
   if (warp == 1) {
     pair_tmem_alloc(tmem_slot, TMEM_COLS);
@@ -179,14 +197,27 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant_
     m0 = (first + r % rows) * 256;
     n0 = (r / rows) * a.bn;
   };
+  // with adapters: the section of a tile, whose n0 counts from the section's start
+  auto section_at = [&](int& n0) {
+    int s = 0;
+    if (!a.dual) {
+      const int tile = n0 / a.bn;
+      while (s + 1 < d.sections && tile >= d.first_tile[s + 1]) ++s;
+      n0 = d.start[s] + (tile - d.first_tile[s]) * a.bn;
+    }
+    return s;
+  };
+  // panels of a token tile that reach a tile of features: of its section, or of the gate and the up half of a gated unit
+  auto panels_of = [&](int m0) { return min(d.counts[m0 / 256], d.capacity) * (a.dual ? d.all_panels : d.panels); };
 
   if (warp == 0) {
     if (elect_one()) {
       int s = 0, early = 0;        // ring stage; k-blocks whose weight tile is already under way
       uint32_t parity = 1;         // of the empty barrier: a fresh one counts as free
       bool ok = true, reused = false;  // reused: the ring has gone round, its stages are free when the MMAs say so
-      int m0, n0, kb0, kb1;
+      int m0, n0, kb0, kb1, section = 0;
       tile_at(pair, m0, n0, kb0, kb1);
+      if (ADAPTERS) section = section_at(n0);
       // the first ring of weight tiles depends on no earlier kernel
       const int pre = min(stages, kb1 - kb0);
       auto load_w = [&](int s, int kb, int n0) {
@@ -198,6 +229,11 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant_
       pdl_wait();  // activations come from the previous kernel
       for (int tile = pair; tile < num_tiles && ok; tile += pairs) {
         tile_at(tile, m0, n0, kb0, kb1);
+        int extra = 0;
+        if (ADAPTERS) {
+          section = section_at(n0);
+          extra = panels_of(m0);
+        }
         for (int kb = kb0; kb < kb1; ++kb) {
           ok = pair_wait(&empty[s], parity, 1);
           if (!ok) break;
@@ -206,6 +242,35 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant_
           else load_w(s, kb, n0);
           pair_tma_load_2d(smem + (size_t)s * stage_bytes, &tmX, cluster_addr(&full[s], 0), kb * 64, m0 + (int)rank * 128);
           if (++s == stages) s = 0, parity ^= 1, reused = true;
+        }
+        if (ADAPTERS) {
+          const int per = a.dual ? d.all_panels : d.panels;
+          const int* const list = d.lists + (size_t)(m0 / 256) * d.capacity;
+          for (int e0 = 0; e0 < extra && ok; e0 += 4) {
+            const int n = min(4, extra - e0);
+            int slot[4];   // asked for before the wait
+#pragma unroll
+            for (int i = 0; i < 4; ++i) slot[i] = i < n ? list[(e0 + i) / per] : 0;
+            ok = pair_wait(&empty[s], parity, 1);
+            if (!ok) break;
+            if (rank == 0 && reused) mbar_arrive_cluster_relaxed(cluster_addr(&empty[s], 1));
+            if (rank == 0) mbar_expect_tx(&full[s], 2 * n * (128 * 32 + a.bn * 16));
+            uint8_t* const st = smem + (size_t)s * stage_bytes;
+            const uint32_t bar = cluster_addr(&full[s], 0);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (i < n) {
+                const int j = (e0 + i) / per, q = (e0 + i) - j * per;   // the adapter, the panel among those of the tile
+                const int of = a.dual ? q : section * d.panels + q, rp = of % d.panels;
+                pair_tma_load_2d(st + i * 4096, &tmH, bar, 0, ((m0 / 256 * d.capacity + j) * d.all_panels + of) * 256 + (int)rank * 128);
+                int row = (slot[i] * d.panels + rp) * d.b_rows;
+                if (!a.dual) row += n0 + (int)rank * (a.bn / 2);
+                else if (of / d.panels == (int)rank) row += n0 / 2 + (rank ? a.up_row : 0);
+                else row = d.no_row;   // a gate's panel adds nothing to the up half, and the other way round
+                pair_tma_load_2d(st + A_BYTES + i * a.bn * 16, &tmB, bar, 0, row);
+              }
+            if (++s == stages) s = 0, parity ^= 1, reused = true;
+          }
         }
       }
       if (!ok && rank == 0) {
@@ -222,6 +287,7 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant_
       int s = 0, local = 0;
       uint32_t parity = 0;
       bool ok = true;
+      if (ADAPTERS) pdl_wait();   // counts come from the previous kernels
       for (int tile = pair; tile < num_tiles && ok; tile += pairs, ++local) {
         const int buf = local & 1;
         if (local >= 2) {
@@ -232,6 +298,7 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant_
         const uint32_t acc = tmem_base + buf * BUF_COLS;
         int m0, n0, kb0, kb1;
         tile_at(tile, m0, n0, kb0, kb1);
+        const int extra = ADAPTERS ? panels_of(m0) : 0;
         for (int kb = kb0; kb < kb1; ++kb) {
           ok = mbar_wait(&full[s], parity, 2);
           if (!ok) break;
@@ -242,6 +309,18 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant_
           for (int k = 0; k < 4; ++k) pair_mma(acc, da + 2 * k, db + 2 * k, idesc, kb != kb0 || k != 0);
           pair_commit(&empty[s]);
           if (++s == stages) s = 0, parity ^= 1;
+        }
+        if (ADAPTERS) {
+          for (int e0 = 0; e0 < extra && ok; e0 += 4) {
+            ok = mbar_wait(&full[s], parity, 2);
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t st = smem_u32(smem + (size_t)s * stage_bytes);
+            for (int i = 0; i < min(4, extra - e0); ++i)
+              pair_mma(acc, umma_desc_sw32(st + i * 4096), umma_desc_sw32(st + A_BYTES + i * a.bn * 16), idesc, 1);
+            pair_commit(&empty[s]);
+            if (++s == stages) s = 0, parity ^= 1;
+          }
         }
         if (ok) pair_commit(&acc_full[buf]);
       }
@@ -257,7 +336,9 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant_
       int m0, n0, kb0, kb1;
       tile_at(tile, m0, n0, kb0, kb1);
       // outputs of this tile: f0 + [0, width); the two warps of a lane quarter take half of the columns each, up to 64 at a time
-      const int f0 = a.dual ? n0 / 2 : n0, full_width = a.dual ? a.bn / 2 : a.bn, width = min(full_width, (a.dual ? a.N / 2 : a.N) - f0);
+      const int section = ADAPTERS ? section_at(n0) : 0;
+      const int f0 = a.dual ? n0 / 2 : n0, full_width = a.dual ? a.bn / 2 : a.bn;
+      const int width = min(full_width, (a.dual ? a.N / 2 : ADAPTERS ? d.end[section] : a.N) - f0);
       const int u_end = min(width, (half + 1) * (full_width / 2));
       const int row0 = m0 + (int)rank * 128 + q * 32;  // first token of this warp
       if (!pair_wait(&acc_full[buf], (uint32_t)(local >> 1) & 1, 3)) break;
@@ -380,4 +461,15 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant_
     tc_fence_after();
     pair_tmem_dealloc(tmem_base, TMEM_COLS);
   }
+}
+
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
+gemm_pair_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW, const PairArgs a) {
+  gemm_pair_body<false>(tmX, tmW, tmX, tmW, a, PairAdapters{});
+}
+
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
+gemm_pair_adapter_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmH,
+                         const __grid_constant__ CUtensorMap tmB, const PairArgs a, const PairAdapters d) {
+  gemm_pair_body<true>(tmX, tmW, tmH, tmB, a, d);
 }

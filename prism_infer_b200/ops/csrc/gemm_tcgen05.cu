@@ -912,6 +912,81 @@ int prism_make_head_tensor_map(const void* ptr, unsigned long long tokens, unsig
   return r == CUDA_SUCCESS ? 0 : -102 - (int)r;
 }
 
+int prism_make_panel_tensor_map(const void* ptr, unsigned long long rows, unsigned box_rows, CUtensorMap* out) {
+  EncodeTiledFn fn = get_encode_fn();
+  if (!fn) return -100;
+  if (reinterpret_cast<uintptr_t>(ptr) & 15) return -101;
+  cuuint64_t dims[2] = {16, rows};
+  cuuint64_t strides[1] = {32};
+  cuuint32_t box[2] = {16, box_rows};
+  cuuint32_t estr[2] = {1, 1};
+  CUresult r = fn(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(ptr), dims, strides, box, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_32B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? 0 : -102 - (int)r;
+}
+
+// The pairs' epilogue moves whole 16-byte vectors of 16 features at a time, from the start of every section.
+bool prism_adapter_pair_fits(int M, int dual, const PrismAdapterTerms& t, const void* out, long long ldo, const void* bias) {
+  const unsigned long long addr = reinterpret_cast<unsigned long long>(out) | reinterpret_cast<unsigned long long>(bias);
+  if ((addr & 15ull) || ldo % 8 || (dual ? M / 2 : M) % 16) return false;
+  for (int s = 0; s < t.sec.n; ++s)
+    if (t.sec.end[s] % 16) return false;
+  return true;
+}
+
+// W [M, K], X [T, K] bf16; out bf16 [T, ldo].  dual: W is gate rows and up rows, M / 2 each, out is act(gate) * up.
+int prism_adapter_pair(const void* W, const void* X, void* out, int M, int T, int K, long long ldw, long long ldx, long long ldo,
+                       const void* bias, int dual, int act, const PrismAdapterTerms& t, cudaStream_t stream, bool pdl) {
+  PairArgs a = {};
+  a.T = T;
+  a.N = M;
+  a.kb_total = (K + BK - 1) / BK;
+  a.splits = 1;
+  a.kb_per_split = a.kb_total;
+  a.dual = dual;
+  a.up_row = M / 2;
+  a.act = act;
+  a.ldo = ldo;
+  a.bias = reinterpret_cast<const __nv_bfloat16*>(bias);
+  a.out = out;
+  a.sec.n = 0;
+  a.m_tiles = (T + 255) / 256;
+  PairAdapters d = {};
+  d.lists = t.lists;
+  d.counts = t.counts;
+  d.capacity = t.capacity;
+  d.panels = t.panels;
+  d.all_panels = t.panels * t.sec.n;
+  d.b_rows = M;
+  d.no_row = t.slots * t.panels * M;
+  d.sections = t.sec.n;
+  a.bn = pair_columns(a.m_tiles, M, dual != 0);
+  a.n_tiles = 0;
+  for (int s = 0; s < t.sec.n; ++s) {
+    d.start[s] = s == 0 ? 0 : t.sec.end[s - 1];
+    d.end[s] = t.sec.end[s];
+    d.first_tile[s] = a.n_tiles;
+    a.n_tiles += (d.end[s] - d.start[s] + a.bn - 1) / a.bn;
+  }
+  if (dual) a.n_tiles = (M + a.bn - 1) / a.bn;
+  const int stage_bytes = W_TILE_BYTES + a.bn * 64;
+  a.stages = (SMEM_LIMIT - 1024 - 512 - PAIR_TURN_BYTES) / stage_bytes;
+  if (a.stages > 12) a.stages = 12;
+  const size_t smem = (size_t)a.stages * stage_bytes + PAIR_TURN_BYTES + 1024 + (2 * a.stages + 4) * 8 + 64;
+  CUtensorMap tx, tw, th, tb;
+  int rc = get_tensor_map(X, (unsigned long long)T, (unsigned long long)K, (unsigned long long)ldx, 128, &tx);
+  if (!rc) rc = get_tensor_map(W, (unsigned long long)M, (unsigned long long)K, (unsigned long long)ldw, (unsigned)(a.bn / 2), &tw);
+  if (!rc) rc = prism_make_panel_tensor_map(t.h, (unsigned long long)t.tiles * t.capacity * d.all_panels * 256, 128, &th);
+  if (!rc) rc = prism_make_panel_tensor_map(t.b, (unsigned long long)t.slots * t.panels * M, (unsigned)(a.bn / 2), &tb);
+  if (rc) return rc;
+  const cudaError_t e = cudaFuncSetAttribute(gemm_pair_adapter_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_LIMIT);
+  if (e != cudaSuccess) return (int)e;
+  const int tiles = a.m_tiles * a.n_tiles, pairs = sm_count() / 2;
+  return (int)prism_launch(gemm_pair_adapter_kernel, dim3(2 * (tiles < pairs ? tiles : pairs)), dim3(PAIR_THREADS), smem, stream, pdl, tx, tw, th, tb,
+                           a, d);
+}
+
 // W [w_rows_total, K] (row stride ldw), X [T, K] (row stride ldx), both bf16.
 // out: bf16 [T, ldo] (features along the row) or fp32 [splits][T][ldo] when out_f32.
 // dual: second weight tile starts at row w2_row_off; output = silu(W1 x) * (W2 x), M rows.

@@ -81,6 +81,7 @@ _SIGNATURES = {
     "prism_adapter_plan": "piiippppi",
     "prism_adapter_shrink": "ippppp" "iiiilpi",
     "prism_adapter_expand": "ipppppp" "iiiiipilpi",
+    "prism_adapter_linear": "ppppp" "pppp" "pp" "iiiiii" "piii" "lllpi",
     "prism_sample": "pllipppiilupppipi",
     "prism_merge_candidates": "pppiipi",
     "prism_lm_head_fp8_plan": "p",
