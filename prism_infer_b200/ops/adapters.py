@@ -29,8 +29,9 @@ MAX_RANK = 256
 
 class AdapterPool:
     """Factors of one projection ``[sum(sections), in_features]`` for up to ``slots`` adapters of rank up to ``rank`` per section, laid
-    out as the kernels read them: ``a [slots, sections * panels * 16, in_features]``, ``b [slots, panels, features, 16]``,
-    ``scale [slots]``.  A slot that was never loaded adds nothing."""
+    out as the kernels read them: ``a [slots, sections * panels * 16, in_features]``, ``b [slots, panels, rows, 16]`` with every section's
+    features padded to a multiple of 8 rows (in bf16 the ranks of 8 rows as ``[2, 8 rows, 8 ranks]``), ``scale [slots]``.  A slot that was
+    never loaded adds nothing."""
 
     def __init__(self, slots: int, rank: int, in_features: int, sections: Union[int, Sequence[int]], *, device,
                  dtype: torch.dtype = torch.bfloat16):
@@ -47,10 +48,11 @@ class AdapterPool:
         self.features = sum(sections)
         self.panels = -(-rank // PANEL)
         self.low = len(sections) * self.panels * PANEL
-        if slots * self.low >= 2 ** 31 or slots * self.panels * self.features >= 2 ** 31:
+        self.rows = sum(-(-m // 8) * 8 for m in sections)
+        if slots * self.low >= 2 ** 31 or slots * self.panels * self.rows >= 2 ** 31:
             raise ValueError("the pool's rows must fit 31 bits")
         self.a = torch.zeros(slots, self.low, in_features, dtype=dtype, device=device)
-        self.b = torch.zeros(slots, self.panels, self.features, PANEL, dtype=dtype, device=device)
+        self.b = torch.zeros(slots, self.panels, self.rows, PANEL, dtype=dtype, device=device)
         self.scale = torch.zeros(slots, dtype=torch.float32, device=device)
         self.device = self.a.device
         ends = [sum(sections[:i + 1]) for i in range(len(sections))]
@@ -78,11 +80,24 @@ class AdapterPool:
         for i, (fa, fb, m) in enumerate(zip(a, b, self.sections)):
             r, row = fa.shape[0], i * self.panels * PANEL
             self.a[slot, row:row + r] = fa
-            padded = torch.zeros(m, self.panels * PANEL, dtype=self.dtype, device=self.device)
-            padded[:, :r] = fb
-            self.b[slot, :, first:first + m] = padded.view(m, self.panels, PANEL).transpose(0, 1)
-            first += m
+            rows = -(-m // 8) * 8
+            padded = torch.zeros(rows, self.panels * PANEL, dtype=self.dtype, device=self.device)
+            padded[:m, :r] = fb
+            self.b[slot, :, first:first + rows] = self._panels(padded.view(rows, self.panels, PANEL).transpose(0, 1))
+            first += rows
         self.scale[slot] = scale
+
+    def _panels(self, b: torch.Tensor) -> torch.Tensor:
+        """``[panels, rows, 16]`` in the pool's order."""
+        return b if self.dtype != torch.bfloat16 else b.reshape(b.shape[0], -1, 8, 2, 8).transpose(2, 3).reshape(b.shape)
+
+    def _features(self, slot: int, section: int) -> torch.Tensor:
+        """``[features of the section, panels * 16]`` from the pool's order."""
+        first, m = sum(-(-n // 8) * 8 for n in self.sections[:section]), self.sections[section]
+        b = self.b[slot, :, first:first + -(-m // 8) * 8]
+        if self.dtype == torch.bfloat16:
+            b = b.reshape(b.shape[0], -1, 2, 8, 8).transpose(2, 3).reshape(b.shape)
+        return b.transpose(0, 1).reshape(b.shape[1], -1)[:m]
 
     def clear(self, slot: int) -> None:
         """The slot adds nothing from here on."""
@@ -169,8 +184,7 @@ def _adapted_cpu(x, w, pool, p, bias):
         low = F.linear(x[rows].float(), pool.a[s].float()) * pool.scale[s]
         first, r = 0, pool.panels * PANEL
         for i, m in enumerate(pool.sections):
-            b = pool.b[s, :, first:first + m].transpose(0, 1).reshape(m, r).float()
-            y[rows, first:first + m] += F.linear(low[:, i * r:(i + 1) * r], b)
+            y[rows, first:first + m] += F.linear(low[:, i * r:(i + 1) * r], pool._features(s, i).float())
             first += m
     return y
 

@@ -3,7 +3,8 @@
 // with stacked W: the features of section s have factors A_a^s, B_a^s of their own.
 //
 // Pools (ops/adapters.py) hold the factors of all loaded adapters with ranks padded to panels of 16: A as rows of K, panel after panel,
-// section after section; B as [slot][panel of a section][feature][16], so that the 16 ranks of a run of features are one piece of memory.
+// section after section; B as [slot][panel of a section][feature][16], every section's features padded to a multiple of 8, in bf16 with the
+// 16 ranks of 8 features as [2][8 features][8 ranks], the order in which the matrix instructions read them.
 #include "common.cuh"
 
 #include <atomic>
@@ -98,12 +99,12 @@ __global__ void __launch_bounds__(256) adapter_shrink_kernel(const ShrinkArgs a)
 struct ExpandArgs {
   const float* base;    // [T][M] W x
   const float* h;       // [T][low]
-  const void* b;        // [slots][panels][M][16]
+  const void* b;        // [slots][panels][b_rows][16]
   const void* bias;     // [M] (null: none)
   const int* adapter;   // [T]
   void* out;            // [T][ldo]
-  int T, M, low, panels, slots, sections;
-  int end[MAX_SECTIONS];
+  int T, M, low, panels, slots, sections, b_rows;
+  int end[MAX_SECTIONS], shift[MAX_SECTIONS];   // shift: of a section's features in b
   int gated;            // silu / gelu of the first half times the second half (PRISM_GLU_*), 0: plain
   long long ldo;
 };
@@ -118,7 +119,7 @@ __device__ __forceinline__ float adapted(const ExpandArgs& a, int t, int m, int 
   const float* const h = a.h + (size_t)t * a.low + s * a.panels * 16;
   float sum = 0.0f;
   for (int p = 0; p < a.panels; ++p) {
-    const T* const b = (const T*)a.b + (((size_t)who * a.panels + p) * a.M + m) * 16;
+    const T* const b = (const T*)a.b + (((size_t)who * a.panels + p) * a.b_rows + m + a.shift[s]) * 16;
 #pragma unroll
     for (int r = 0; r < 16; ++r) sum += h[p * 16 + r] * to_float(b[r]);
   }
@@ -173,8 +174,8 @@ __device__ __forceinline__ uint2 pack4(const float4& v) {
 // Share z of a sum over kb k-blocks in CS parts, none of them empty (CS <= kb).
 __device__ __forceinline__ int part_begin(int kb, int z, int cs) { return (int)((long long)kb * z / cs); }
 
-// One token's 128 sums of the accumulator (lane = row) to shared memory, token after token.
-template <int BN>
+// The accumulator's 128 rows (lanes) of every token to shared memory, token after token.
+template <int BN, int PITCH>
 __device__ __forceinline__ void accumulator_to_smem(uint32_t tmem, float* red, int q, int lane, int tokens) {
   const uint32_t t_lane = tmem + ((uint32_t)(q * 32) << 16);
   for (int c0 = 0; c0 < tokens; c0 += 16) {
@@ -182,7 +183,7 @@ __device__ __forceinline__ void accumulator_to_smem(uint32_t tmem, float* red, i
     tmem_ld16(t_lane + c0, r);
     tmem_ld_wait();
 #pragma unroll
-    for (int j = 0; j < 16; ++j) red[(c0 + j) * RED_PITCH + q * 32 + lane] = __uint_as_float(r[j]);
+    for (int j = 0; j < 16; ++j) red[(c0 + j) * PITCH + q * 32 + lane] = __uint_as_float(r[j]);
   }
 }
 
@@ -191,26 +192,85 @@ struct LowArgs {
   const int* counts;     // [tiles]
   const int* index;      // [T]
   const float* scale;    // [slots]
-  bf16* h;               // [tiles][capacity][all_panels][tile_rows][16]
+  bf16* h;               // [tiles][capacity][all_panels] panels of tile_rows tokens
   int T, kb, capacity, all_panels, tile_rows, stages;
 };
 
-// h of one tile of BN tokens: cluster (1, 1, CS) splits K, its CTAs add their sums through one another's shared memory.
-template <int BN>
+// The place of every token of a tile in the list of adapters, and that adapter's scale.
+template <int TOKENS>
+__device__ __forceinline__ void load_owners(const LowArgs& a, int* who, float* scale, int token0, const int* list) {
+  for (int c = threadIdx.x; c < TOKENS; c += TC_THREADS) {
+    const int j = token0 + c < a.T ? a.index[token0 + c] : -1;
+    who[c] = j;
+    scale[c] = j >= 0 ? a.scale[list[j]] : 0.0f;
+  }
+}
+
+// Sum over the cluster of four floats that every CTA keeps at the same place.
+__device__ __forceinline__ float4 cluster_sum4(const float* mine, int cs) {
+  const uint32_t at = smem_u32(mine);
+  float4 v[8];
+#pragma unroll
+  for (int peer = 0; peer < 8; ++peer)
+    if (peer < cs) {
+      uint32_t remote;
+      asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(at), "r"(peer));
+      v[peer] = ld_cluster4(remote);
+    }
+#pragma unroll
+  for (int peer = 1; peer < 8; ++peer)
+    if (peer < cs) v[0] = add4(v[0], v[peer]);
+  return v[0];
+}
+
+// Where ranks 8 * half .. + 8 of a panel's row lie.
+__device__ __forceinline__ size_t in_panel(int row, int half) { return (size_t)(row >> 3) * 128 + half * 64 + (row & 7) * 8; }
+
+// Panels of h from the sums in `red`, of which every CTA of the cluster holds a part: each CTA adds up and stores its share of the tokens,
+// zeros in panels of adapters that are not the token's.  panel_at(g) is the g-th of the np panels.
+template <int PITCH, bool TOKEN_MAJOR, int TOKENS, typename PanelAt>
+__device__ __forceinline__ void store_low_rows(const LowArgs& a, const float* red, const int* who, const float* scale, PanelAt panel_at, int np, int token0,
+                                               int tile) {
+  const int cs = gridDim.z, share = TOKENS / cs, first = blockIdx.z * share, shift = __ffs(share) - 1;   // a power of two
+  bf16* const h = a.h + (size_t)tile * a.capacity * a.all_panels * a.tile_rows * 16;
+  for (int i = threadIdx.x; i < np * share * 2; i += TC_THREADS) {   // items of eight ranks
+    const int half = (i >> shift) & 1, c = first + (i & (share - 1)), g = i >> (1 + shift), p = panel_at(g), own = p - who[c] * a.all_panels;
+    uint4 o = make_uint4(0, 0, 0, 0);
+    if (who[c] >= 0 && own >= 0 && own < a.all_panels) {
+      const float* const mine = red + (TOKEN_MAJOR ? c * PITCH + g * 16 : (g * TOKENS + c) * PITCH) + half * 8;
+      const float4 v = cluster_sum4(mine, cs), u = cluster_sum4(mine + 4, cs);
+      const float f = scale[c];
+      const uint2 lo = pack4(make_float4(v.x * f, v.y * f, v.z * f, v.w * f)), hi = pack4(make_float4(u.x * f, u.y * f, u.z * f, u.w * f));
+      o = make_uint4(lo.x, lo.y, hi.x, hi.y);
+    }
+    *reinterpret_cast<uint4*>(h + (size_t)p * a.tile_rows * 16 + in_panel(token0 - tile * PLAN_TILE + c, half)) = o;
+  }
+}
+
+// Decode steps, one tile of BN tokens: the panels' rows of A are the MMA's 128 rows (G runs of eight panels at a time), the tokens its
+// columns.  Cluster (1, 1, CS) splits K.
+template <int BN, int G>
 __global__ void __launch_bounds__(TC_THREADS, 1)
 adapter_low_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmX, const LowArgs a) {
-  constexpr int TMEM_COLS = BN < 32 ? 32 : BN, STAGE = stage_bytes<BN>();
+  constexpr int TMEM_COLS = G * BN < 32 ? 32 : G * BN, X_AT = G * W_BYTES, STAGE = X_AT + BN * 128, PITCH = G * 128 + 4;
+  // The projection starts now: what it reads besides h comes from kernels that are done when the last block is here, so it streams its
+  // weights meanwhile and waits for this kernel only before its panels.
+  pdl_wait();   // tokens and plan come from the previous kernels, and h may still be read by them
+  pdl_launch_dependents();
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  float* const red = reinterpret_cast<float*>(smem);   // the ring's memory, between two groups of panels
+  float* const red = reinterpret_cast<float*>(smem);   // the ring's memory, between two passes
   const int stages = a.stages;
-  const size_t ring = max((size_t)stages * STAGE, (size_t)BN * RED_PITCH * 4);
+  const size_t ring = max((size_t)stages * STAGE, (size_t)BN * PITCH * 4);
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + ring);
   uint64_t* empty = full + stages;
   uint64_t* acc_full = empty + stages;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 1);
   const int warp = uniform_warp(), lane = threadIdx.x & 31;
-  const int cs = gridDim.z, z = blockIdx.z, token0 = blockIdx.y * BN, tile = token0 / PLAN_TILE;
+  const int panels = min(a.counts[0], a.capacity) * a.all_panels;
+  const int* const list = a.lists;
+  __shared__ int who[BN];
+  __shared__ float scale[BN];
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < stages; ++s) {
@@ -226,26 +286,23 @@ adapter_low_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
     tmem_alloc(tmem_slot, TMEM_COLS);
     tmem_relinquish();
   }
+  load_owners<BN>(a, who, scale, 0, list);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  pdl_launch_dependents();
-  pdl_wait();   // tokens and plan come from the previous kernels, and h may still be read by them
 
-  const int panels = min(a.counts[tile], a.capacity) * a.all_panels;
-  const int* const list = a.lists + (size_t)tile * a.capacity;
-  const int kb0 = part_begin(a.kb, z, cs), kb1 = part_begin(a.kb, z + 1, cs);
-  int s = 0, round = 0;   // ring stage; groups of panels done
+  const int kb0 = part_begin(a.kb, blockIdx.z, gridDim.z), kb1 = part_begin(a.kb, blockIdx.z + 1, gridDim.z);
+  int s = 0, round = 0;   // ring stage; passes done
   uint32_t parity = 0;    // of the full barriers (MMA); the producer waits for the phase before
   bool ok = true;         // this thread's role goes on; after a wait that ran out it only keeps step with the cluster
-  for (int p0 = blockIdx.x * 8; p0 < panels; p0 += gridDim.x * 8, ++round) {
-    const int np = min(8, panels - p0);
+  for (int p0 = blockIdx.x * G * 8; p0 < panels; p0 += gridDim.x * G * 8, ++round) {
+    const int np = min(G * 8, panels - p0);
     if (warp == 0) {
       if (elect_one() && ok) {
-        int row[8];
+        int row[G * 8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < G * 8; ++i) {
           const int p = p0 + min(i, np - 1), j = p / a.all_panels;
           row[i] = (list[j] * a.all_panels + (p - j * a.all_panels)) * 16;
         }
@@ -254,9 +311,9 @@ adapter_low_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
           if (!ok) break;
           uint8_t* const st = smem + (size_t)s * STAGE;
           mbar_expect_tx(&full[s], np * 2048 + BN * 128);
-          tma_load_2d(st + W_BYTES, &tmX, &full[s], kb * 64, token0);
+          tma_load_2d(st + X_AT, &tmX, &full[s], kb * 64, 0);
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
+          for (int i = 0; i < G * 8; ++i)
             if (i < np) tma_load_2d(st + i * 2048, &tmA, &full[s], kb * 64, row[i]);
           if (++s == stages) s = 0, parity ^= 1;
         }
@@ -276,9 +333,14 @@ adapter_low_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
           if (!ok) break;
           tc_fence_after();
           const uint32_t st = smem_u32(smem + (size_t)s * STAGE);
-          const uint64_t da = umma_desc_sw128(st), db = umma_desc_sw128(st + W_BYTES);
+          const uint64_t db = umma_desc_sw128(st + X_AT);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) tc_mma_f16(tmem, da + 2 * k, db + 2 * k, idesc, kb != kb0 || k != 0);
+          for (int g = 0; g < G; ++g)
+            if (g * 8 < np) {
+              const uint64_t da = umma_desc_sw128(st + g * W_BYTES);
+#pragma unroll
+              for (int k = 0; k < 4; ++k) tc_mma_f16(tmem + g * BN, da + 2 * k, db + 2 * k, idesc, kb != kb0 || k != 0);
+            }
           tc_commit(&empty[s]);
           if (++s == stages) s = 0, parity ^= 1;
         }
@@ -289,27 +351,176 @@ adapter_low_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
       ok = ok && __all_sync(0xffffffffu, mbar_wait(acc_full, round & 1, 3));
       if (ok) {
         tc_fence_after();
-        accumulator_to_smem<BN>(tmem, red, warp & 3, lane, BN);
+        for (int g = 0; g * 8 < np; ++g) accumulator_to_smem<BN, PITCH>(tmem + g * BN, red + g * 128, warp & 3, lane, BN);
       }
     }
     tc_fence_before();
     __syncwarp();
     cluster_sync_all();
     tc_fence_after();
-    // items of four ranks: the ranks of a token's panel fastest, then its tokens; every CTA takes its share of the tokens
-    const int share = BN / cs, first = z * share;
-    for (int i = threadIdx.x; i < np * share * 4; i += TC_THREADS) {
-      const int quarter = i & 3, c = first + (i >> 2) % share, g = (i >> 2) / share, p = p0 + g, j = p / a.all_panels, t = token0 + c;
-      float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      if (t < a.T && a.index[t] == j) {
-        for (int peer = 0; peer < cs; ++peer) v = add4(v, ld_cluster4(cluster_addr(red + c * RED_PITCH + g * 16 + quarter * 4, peer)));
-        const float scale = a.scale[list[j]];
-        v = make_float4(v.x * scale, v.y * scale, v.z * scale, v.w * scale);
-      }
-      const size_t at = (((size_t)tile * a.capacity * a.all_panels + p) * a.tile_rows + (t - tile * PLAN_TILE)) * 16 + quarter * 4;
-      *reinterpret_cast<uint2*>(a.h + at) = pack4(v);
-    }
+    store_low_rows<PITCH, true, BN>(a, red, who, scale, [&](int g) { return p0 + g; }, np, 0, 0);
     // the ring is written again by copies once every CTA has read the sums
+    fence_proxy_async();
+    cluster_sync_all();
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, TMEM_COLS);
+  }
+}
+
+// Prompts, 128 tokens: the tokens are the MMA's rows and up to 16 panels its columns, those of the adapters that these tokens have, so that a
+// k-block moves the tokens once and the factors of these adapters; the panels of the tile's other adapters get zeros.  Cluster (1, 1, CS)
+// splits K.
+__global__ void __launch_bounds__(TC_THREADS, 1)
+adapter_low_prompt_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmX, const LowArgs a) {
+  constexpr int PASS = 16, STAGE = W_BYTES + PASS * 2048, TMEM_COLS = PASS * 16, PITCH = 20;   // 20: rows of 16 floats without bank conflicts
+  pdl_wait();
+  pdl_launch_dependents();   // as above
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  float* const red = reinterpret_cast<float*>(smem);   // [panel of the pass][token][PITCH], in the ring's memory
+  const int stages = a.stages;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + (size_t)stages * STAGE);
+  uint64_t* empty = full + stages;
+  uint64_t* acc_full = empty + stages;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 1);
+  const int warp = uniform_warp(), lane = threadIdx.x & 31;
+  const int token0 = blockIdx.y * 128, tile = token0 / PLAN_TILE;
+  const int count = min(a.counts[tile], a.capacity);
+  const int* const list = a.lists + (size_t)tile * a.capacity;
+  __shared__ int who[128];
+  __shared__ float scale[128];
+  __shared__ short place[PLAN_TILE], active[128];   // of the list's adapters: which of the active ones, -1: none; and back
+  __shared__ int n_active;
+  for (int j = threadIdx.x; j < count; j += TC_THREADS) place[j] = -1;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < stages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    mbar_init(acc_full, 1);
+    fence_barrier_init();
+    tma_prefetch_desc(&tmA);
+    tma_prefetch_desc(&tmX);
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, TMEM_COLS);
+    tmem_relinquish();
+  }
+  load_owners<128>(a, who, scale, token0, list);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  if (threadIdx.x < 128 && who[threadIdx.x] >= 0) place[who[threadIdx.x]] = 0;
+  __syncthreads();
+  if (warp == 2) {
+    int n = 0;
+    for (int j0 = 0; j0 < count; j0 += 32) {
+      const int j = j0 + lane;
+      const bool used = j < count && place[j] >= 0;
+      const unsigned votes = __ballot_sync(0xffffffffu, used);
+      const int at = n + __popc(votes & ((1u << lane) - 1));
+      if (used) {
+        place[j] = (short)at;
+        active[at] = (short)j;
+      }
+      n += __popc(votes);
+    }
+    if (lane == 0) n_active = n;
+  }
+  __syncthreads();
+  const int panels = n_active * a.all_panels;
+  if (warp >= 2) {   // zeros for adapters that only the tile's other 128 tokens have
+    const int cs = gridDim.z, share = 128 / cs;
+    bf16* const h = a.h + (size_t)tile * a.capacity * a.all_panels * a.tile_rows * 16;
+    for (int j = 0; j < count; ++j)
+      if (place[j] < 0)
+        for (int i = threadIdx.x - 64; i < a.all_panels * share * 2; i += 128)
+          *reinterpret_cast<uint4*>(h + ((size_t)j * a.all_panels + i / (share * 2)) * a.tile_rows * 16 +
+                                    in_panel(token0 - tile * PLAN_TILE + blockIdx.z * share + (i >> 1) % share, i & 1)) = make_uint4(0, 0, 0, 0);
+  }
+
+  const int kb0 = part_begin(a.kb, blockIdx.z, gridDim.z), kb1 = part_begin(a.kb, blockIdx.z + 1, gridDim.z);
+  int s = 0, round = 0;
+  uint32_t parity = 0;
+  bool ok = true;
+  for (int p0 = 0; p0 < panels; p0 += PASS, ++round) {
+    const int np = min(PASS, panels - p0);
+    if (warp == 0) {
+      if (elect_one() && ok) {
+        int row[PASS];
+#pragma unroll
+        for (int i = 0; i < PASS; ++i) {
+          const int p = p0 + min(i, np - 1), j = p / a.all_panels;
+          row[i] = (list[active[j]] * a.all_panels + (p - j * a.all_panels)) * 16;
+        }
+        for (int kb = kb0; kb < kb1; ++kb) {
+          ok = mbar_wait(&empty[s], parity ^ 1, 1);
+          if (!ok) break;
+          uint8_t* const st = smem + (size_t)s * STAGE;
+          mbar_expect_tx(&full[s], W_BYTES + np * 2048);
+          tma_load_2d(st, &tmX, &full[s], kb * 64, token0);
+#pragma unroll
+          for (int i = 0; i < PASS; ++i)
+            if (i < np) tma_load_2d(st + W_BYTES + i * 2048, &tmA, &full[s], kb * 64, row[i]);
+          if (++s == stages) s = 0, parity ^= 1;
+        }
+        if (!ok) {
+          for (int j = 0; j < stages; ++j) {
+            if (--s < 0) s = stages - 1, parity ^= 1;
+            (void)mbar_wait(&full[s], parity, 4);
+          }
+        }
+      }
+    } else if (warp == 1) {
+      if (elect_one() && ok) {
+        const uint32_t idesc = umma_idesc_bf16(128, np * 16);
+        for (int kb = kb0; kb < kb1; ++kb) {
+          ok = mbar_wait(&full[s], parity, 2);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t st = smem_u32(smem + (size_t)s * STAGE);
+          const uint64_t da = umma_desc_sw128(st), db = umma_desc_sw128(st + W_BYTES);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) tc_mma_f16(tmem, da + 2 * k, db + 2 * k, idesc, kb != kb0 || k != 0);
+          tc_commit(&empty[s]);
+          if (++s == stages) s = 0, parity ^= 1;
+        }
+        if (ok) tc_commit(acc_full);
+      }
+    } else {
+      const int q = warp & 3, c = q * 32 + lane, first_own = who[c] < 0 ? panels : place[who[c]] * a.all_panels;
+      ok = ok && __all_sync(0xffffffffu, mbar_wait(acc_full, round & 1, 3));
+      if (ok) {
+        tc_fence_after();
+        for (int g = 0; g < np; ++g) {
+          const bool keep = p0 + g >= first_own && p0 + g < first_own + a.all_panels;
+          if (!__any_sync(0xffffffffu, keep)) continue;
+          uint32_t r[16];
+          tmem_ld16(tmem + ((uint32_t)(q * 32) << 16) + g * 16, r);
+          tmem_ld_wait();
+          float4* const dst = reinterpret_cast<float4*>(red + (g * 128 + c) * PITCH);
+          if (keep)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              dst[e] = make_float4(__uint_as_float(r[4 * e]), __uint_as_float(r[4 * e + 1]), __uint_as_float(r[4 * e + 2]), __uint_as_float(r[4 * e + 3]));
+        }
+      }
+    }
+    tc_fence_before();
+    __syncwarp();
+    cluster_sync_all();
+    tc_fence_after();
+    auto panel_at = [&](int g) {
+      const int k = (p0 + g) / a.all_panels;
+      return active[k] * a.all_panels + (p0 + g - k * a.all_panels);
+    };
+    store_low_rows<PITCH, false, 128>(a, red, who, scale, panel_at, np, token0, tile);
     fence_proxy_async();
     cluster_sync_all();
   }
@@ -329,10 +540,10 @@ struct TileArgs {
   long long ldo;
   int T, M, kb, capacity, panels, all_panels, tile_rows, stages;
   int act;               // DUAL: PRISM_GLU_*
-  int no_row;            // a row behind all of B, which reads as zeros
+  int b_groups, no_group;   // groups of 8 features in a panel of B; a group behind all of them, which reads as zeros
   int vec;               // four features of a row can be stored at once
   int sections;
-  int start[MAX_SECTIONS], end[MAX_SECTIONS], first_tile[MAX_SECTIONS];
+  int start[MAX_SECTIONS], end[MAX_SECTIONS], first_tile[MAX_SECTIONS], b_start[MAX_SECTIONS];   // b_start: in groups
 };
 
 // 128 features (DUAL: 64 gates and their 64 ups) of BN tokens.  Weights are the A operand and stream once; cluster (1, 1, CS) splits the
@@ -359,15 +570,23 @@ adapter_gemm_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_consta
   const int f0 = DUAL ? blockIdx.x * FEATURES : a.start[section] + ((int)blockIdx.x - a.first_tile[section]) * FEATURES;
   const int f_end = DUAL ? a.M / 2 : a.end[section];
 
-  if (threadIdx.x == 0) {
+  const int kb0 = part_begin(a.kb, z, cs), kb1 = part_begin(a.kb, z + 1, cs);
+  const int pre = min(stages, kb1 - kb0);
+  auto load_block = [&](int s, int kb) {
+    uint8_t* const st = smem + (size_t)s * STAGE;
+    mbar_expect_tx(&full[s], STAGE);
+    tma_load_2d(st, &tmW, &full[s], kb * 64, f0);
+    if (DUAL) tma_load_2d(st + W_BYTES / 2, &tmW, &full[s], kb * 64, a.M / 2 + f0);
+    tma_load_2d(st + W_BYTES, &tmX, &full[s], kb * 64, token0);
+  };
+  if (warp == 0 && elect_one()) {
     for (int s = 0; s < stages; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
     mbar_init(acc_full, 1);
     fence_barrier_init();
-    tma_prefetch_desc(&tmW);
-    tma_prefetch_desc(&tmX);
+    for (int i = 0; i < pre; ++i) load_block(i, kb0 + i);   // the first ring is under way before anything else is set up
     tma_prefetch_desc(&tmB);
     tma_prefetch_desc(&tmH);
   }
@@ -381,36 +600,33 @@ adapter_gemm_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_consta
   const uint32_t tmem = *tmem_slot;
   pdl_launch_dependents();
 
-  const int kb0 = part_begin(a.kb, z, cs), kb1 = part_begin(a.kb, z + 1, cs);
   const int per = DUAL ? a.all_panels : a.panels;   // panels of one adapter that reach this tile
   if (warp == 0) {
     if (elect_one()) {
-      auto load_w = [&](int s, int kb) {
-        uint8_t* const st = smem + (size_t)s * STAGE;
-        mbar_expect_tx(&full[s], STAGE);
-        tma_load_2d(st, &tmW, &full[s], kb * 64, f0);
-        if (DUAL) tma_load_2d(st + W_BYTES / 2, &tmW, &full[s], kb * 64, a.M / 2 + f0);
-      };
-      const int pre = min(stages, kb1 - kb0);
-      for (int i = 0; i < pre; ++i) load_w(i, kb0 + i);   // weights depend on no earlier kernel
-      pdl_wait();
       const int extra = min(a.counts[tile], a.capacity) * per;
       const int* const list = a.lists + (size_t)tile * a.capacity;
+      // this CTA's panels: adapter j of the list, panel rp of its section (of: of all sections), the slots asked for one adapter ahead
+      const int e_begin = part_begin(extra, z, cs), e_end = part_begin(extra, z + 1, cs), of0 = DUAL ? 0 : section * a.panels;
+      int j = e_begin / per, of = of0 + (e_begin - j * per), rp = of % a.panels, slot = 0, next = 0;
+      if (e_begin < e_end) {
+        slot = list[j];
+        next = list[min(j + 1, a.capacity - 1)];
+      }
+      const int b_at = DUAL ? f0 / 8 : a.b_start[section] + (f0 - a.start[section]) / 8;
       int s = 0;
       uint32_t parity = 1;   // a fresh empty barrier counts as free
       bool ok = true;
       for (int kb = kb0; kb < kb1; ++kb) {
-        ok = mbar_wait(&empty[s], parity, 1);
-        if (!ok) break;
-        if (kb - kb0 >= pre) load_w(s, kb);
-        tma_load_2d(smem + (size_t)s * STAGE + W_BYTES, &tmX, &full[s], kb * 64, token0);
+        if (kb - kb0 >= pre) {
+          ok = mbar_wait(&empty[s], parity, 1);
+          if (!ok) break;
+          load_block(s, kb);
+        }
         if (++s == stages) s = 0, parity ^= 1;
       }
-      for (int e0 = z * 4; e0 < extra && ok; e0 += cs * 4) {
-        const int n = min(4, extra - e0);
-        int slot[4];   // asked for before the wait
-#pragma unroll
-        for (int i = 0; i < 4; ++i) slot[i] = i < n ? list[(e0 + i) / per] : 0;
+      pdl_wait();   // the low-rank rows
+      for (int e0 = e_begin; e0 < e_end && ok; e0 += 4) {
+        const int n = min(4, e_end - e0);
         ok = mbar_wait(&empty[s], parity, 1);
         if (!ok) break;
         uint8_t* const st = smem + (size_t)s * STAGE;
@@ -418,17 +634,26 @@ adapter_gemm_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_consta
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           if (i < n) {
-            const int j = (e0 + i) / per, q = (e0 + i) - j * per, of = DUAL ? q : section * a.panels + q;
-            const int row = (slot[i] * a.panels + of % a.panels) * a.M;
+            const int group = (slot * a.panels + rp) * a.b_groups + b_at;
             if (DUAL) {   // a gate's panel adds nothing to the up half, and the other way round
               const bool up = of >= a.panels;
-              tma_load_2d(st + i * 4096, &tmB, &full[s], 0, up ? a.no_row : row + f0);
-              tma_load_2d(st + i * 4096 + 2048, &tmB, &full[s], 0, up ? row + a.M / 2 + f0 : a.no_row);
+              tma_load_2d(st + i * 4096, &tmB, &full[s], 0, up ? a.no_group : group);
+              tma_load_2d(st + i * 4096 + 2048, &tmB, &full[s], 0, up ? group + a.b_start[1] : a.no_group);
             } else {
-              tma_load_2d(st + i * 4096, &tmB, &full[s], 0, row + f0);
+              tma_load_2d(st + i * 4096, &tmB, &full[s], 0, group);
             }
             tma_load_2d(st + W_BYTES + i * BN * 32, &tmH, &full[s], 0,
-                        ((tile * a.capacity + j) * a.all_panels + of) * a.tile_rows + (token0 - tile * PLAN_TILE));
+                        (((tile * a.capacity + j) * a.all_panels + of) * a.tile_rows + (token0 - tile * PLAN_TILE)) / 8);
+            ++of;
+            if (++rp == a.panels) {
+              rp = 0;
+              if (!DUAL || of == a.all_panels) {
+                of = of0;
+                ++j;
+                slot = next;
+                next = list[min(j + 1, a.capacity - 1)];
+              }
+            }
           }
         if (++s == stages) s = 0, parity ^= 1;
       }
@@ -443,7 +668,6 @@ adapter_gemm_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_consta
   } else if (warp == 1) {
     if (elect_one()) {
       constexpr uint32_t idesc = umma_idesc_bf16(128, BN);
-      pdl_wait();   // the number of panels comes from the previous kernels
       const int extra = min(a.counts[tile], a.capacity) * per;
       int s = 0;
       uint32_t parity = 0;
@@ -459,12 +683,14 @@ adapter_gemm_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_consta
         tc_commit(&empty[s]);
         if (++s == stages) s = 0, parity ^= 1;
       }
-      for (int e0 = z * 4; e0 < extra && ok; e0 += cs * 4) {
+      const int e_end = part_begin(extra, z + 1, cs);
+      for (int e0 = part_begin(extra, z, cs); e0 < e_end && ok; e0 += 4) {
         ok = mbar_wait(&full[s], parity, 2);
         if (!ok) break;
         tc_fence_after();
         const uint32_t st = smem_u32(smem + (size_t)s * STAGE);
-        for (int i = 0; i < min(4, extra - e0); ++i) tc_mma_f16(tmem, umma_desc_sw32(st + i * 4096), umma_desc_sw32(st + W_BYTES + i * BN * 32), idesc, 1);
+        for (int i = 0; i < min(4, e_end - e0); ++i)
+          tc_mma_f16(tmem, umma_desc_panel(st + i * 4096), umma_desc_panel(st + W_BYTES + i * BN * 32), idesc, 1);
         tc_commit(&empty[s]);
         if (++s == stages) s = 0, parity ^= 1;
       }
@@ -474,7 +700,7 @@ adapter_gemm_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_consta
     pdl_wait();
     if (__all_sync(0xffffffffu, mbar_wait(acc_full, 0, 3))) {
       tc_fence_after();
-      accumulator_to_smem<BN>(tmem, red, warp & 3, lane, min(BN, a.T - token0));
+      accumulator_to_smem<BN, RED_PITCH>(tmem, red, warp & 3, lane, min(BN, a.T - token0));
     }
   }
   tc_fence_before();
@@ -486,15 +712,10 @@ adapter_gemm_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_consta
   for (int i = part_begin(items, z, cs) + threadIdx.x; i < part_begin(items, z + 1, cs); i += TC_THREADS) {
     const int c = i / QUADS, f = f0 + (i % QUADS) * 4, n = min(4, f_end - f);
     if (n <= 0) continue;
-    auto sum_at = [&](int row) {
-      float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      for (int peer = 0; peer < cs; ++peer) v = add4(v, ld_cluster4(cluster_addr(red + c * RED_PITCH + row, peer)));
-      return v;
-    };
-    float4 v = sum_at((i % QUADS) * 4);
+    float4 v = cluster_sum4(red + c * RED_PITCH + (i % QUADS) * 4, cs);
     float* const x = &v.x;
     if (DUAL) {
-      const float4 u = sum_at(64 + (i % QUADS) * 4);
+      const float4 u = cluster_sum4(red + c * RED_PITCH + 64 + (i % QUADS) * 4, cs);
       v = make_float4(glu(v.x, u.x, a.act), glu(v.y, u.y, a.act), glu(v.z, u.z, a.act), glu(v.w, u.w, a.act));
     } else if (a.bias != nullptr) {
       for (int e = 0; e < n; ++e) x[e] += __bfloat162float(a.bias[f + e]);
@@ -513,7 +734,7 @@ adapter_gemm_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_consta
 }
 
 constexpr int SMS = 148;
-constexpr int SMEM_LIMIT = 232448;   // 227 KB
+constexpr int SMEM_LIMIT = 232448 - 2048;   // 227 KB, 2 KB of it for static arrays
 
 // Dynamic shared memory above 48 KB has to be allowed once per kernel and device.
 template <typename Kernel>
@@ -528,14 +749,13 @@ cudaError_t allow_smem(Kernel kernel, std::atomic<unsigned long long>& devices) 
   return e;
 }
 
-// Ring stages in `budget` bytes, and the whole of the dynamic shared memory.
-template <int BN>
-int ring_stages(int budget, size_t& smem) {
-  int stages = (budget - 1024 - 256) / stage_bytes<BN>();
+// Ring stages of `stage` bytes in `budget` bytes, the sums of `red` bytes in the same memory, and the whole of the dynamic shared memory.
+int ring_stages(int budget, int stage, size_t red, size_t& smem) {
+  int stages = (budget - 1024 - 256) / stage;
   if (stages > 12) stages = 12;
   if (stages < 2) stages = 2;
-  size_t ring = (size_t)stages * stage_bytes<BN>();
-  if (ring < (size_t)BN * RED_PITCH * 4) ring = (size_t)BN * RED_PITCH * 4;
+  size_t ring = (size_t)stages * stage;
+  if (ring < red) ring = red;
   smem = 1024 + ring + (2 * stages + 1) * 8 + 16;
   return stages;
 }
@@ -560,27 +780,47 @@ struct Call {
   bool pdl;
 };
 
-template <int BN>
+constexpr int HALF_SM = 112 * 1024;   // two such blocks share an SM: the projection's first loads overlap the low-rank rows
+
+LowArgs low_args(const Call& c) {
+  return LowArgs{c.terms.lists, c.terms.counts, c.index, c.scale, (bf16*)c.h, c.T, (c.K + 63) / 64, c.terms.capacity, c.terms.panels * c.terms.sec.n,
+                 c.tile_rows, 0};
+}
+
+template <int BN, int G>
 int launch_low(const Call& c) {
   static std::atomic<unsigned long long> devices{0};
-  cudaError_t e = allow_smem(adapter_low_kernel<BN>, devices);
+  cudaError_t e = allow_smem(adapter_low_kernel<BN, G>, devices);
   if (e != cudaSuccess) return (int)e;
-  const int all = c.terms.panels * c.terms.sec.n, tiles = (c.T + BN - 1) / BN;
-  LowArgs a{c.terms.lists, c.terms.counts, c.index, c.scale, (bf16*)c.h, c.T, (c.K + 63) / 64, c.terms.capacity, all, c.tile_rows, 0};
-  // A decode step may bring as many adapters as tokens; the tiles of a prompt hold runs of a few requests.
-  const int groups = c.T <= 128 ? (c.terms.capacity * all + 7) / 8 : 1;
-  int cs = power_below(SMS / (groups * tiles > SMS ? SMS : groups * tiles));
+  LowArgs a = low_args(c);
+  const int most = (a.capacity * a.all_panels + G * 8 - 1) / (G * 8);   // a step may bring as many adapters as tokens
+  int cs = power_below(SMS / (most > SMS ? SMS : most));
   if (cs > a.kb) cs = power_below(a.kb);
-  const int gx = SMS / (tiles * cs);
+  const int gx = SMS / cs < most ? SMS / cs : most;
   size_t smem;
-  a.stages = ring_stages<BN>(113 * 1024, smem);
+  a.stages = ring_stages(G == 1 ? HALF_SM : SMEM_LIMIT, G * W_BYTES + BN * 128, (size_t)BN * (G * 128 + 4) * 4, smem);
   CUtensorMap ta, tx;
-  int rc = prism_get_tensor_map(c.a, (unsigned long long)c.terms.slots * all * 16, (unsigned long long)c.K, (unsigned long long)c.K, 16, &ta);
+  int rc = prism_get_tensor_map(c.a, (unsigned long long)c.terms.slots * a.all_panels * 16, (unsigned long long)c.K, (unsigned long long)c.K, 16, &ta);
   if (!rc) rc = prism_get_tensor_map(c.x, (unsigned long long)c.T, (unsigned long long)c.K, (unsigned long long)c.ldx, BN, &tx);
   if (rc) return rc;
-  const int most = (c.terms.capacity * all + 7) / 8;
-  return (int)prism_launch_clusters(adapter_low_kernel<BN>, dim3(gx < 1 ? 1 : gx < most ? gx : most, tiles, cs), dim3(TC_THREADS), smem, c.stream,
-                                    c.pdl, cs, ta, tx, a);
+  return (int)prism_launch_clusters(adapter_low_kernel<BN, G>, dim3(gx, 1, cs), dim3(TC_THREADS), smem, c.stream, c.pdl, cs, ta, tx, a);
+}
+
+int launch_low_prompt(const Call& c) {
+  static std::atomic<unsigned long long> devices{0};
+  cudaError_t e = allow_smem(adapter_low_prompt_kernel, devices);
+  if (e != cudaSuccess) return (int)e;
+  LowArgs a = low_args(c);
+  const int tiles = (c.T + 127) / 128;
+  int cs = power_below(SMS / (tiles > SMS ? SMS : tiles));
+  if (cs > a.kb) cs = power_below(a.kb);
+  size_t smem;
+  a.stages = ring_stages(SMEM_LIMIT, W_BYTES + 16 * 2048, (size_t)16 * 128 * 20 * 4, smem);
+  CUtensorMap ta, tx;
+  int rc = prism_get_tensor_map(c.a, (unsigned long long)c.terms.slots * a.all_panels * 16, (unsigned long long)c.K, (unsigned long long)c.K, 16, &ta);
+  if (!rc) rc = prism_get_tensor_map(c.x, (unsigned long long)c.T, (unsigned long long)c.K, (unsigned long long)c.ldx, 128, &tx);
+  if (rc) return rc;
+  return (int)prism_launch_clusters(adapter_low_prompt_kernel, dim3(1, tiles, cs), dim3(TC_THREADS), smem, c.stream, c.pdl, cs, ta, tx, a);
 }
 
 template <int BN, bool DUAL>
@@ -605,13 +845,15 @@ int launch_tiles(const Call& c) {
   a.all_panels = all;
   a.tile_rows = c.tile_rows;
   a.act = c.act;
-  a.no_row = t.slots * t.panels * c.M;
+  a.b_groups = t.b_rows / 8;
+  a.no_group = t.slots * t.panels * a.b_groups;
   a.sections = t.sec.n;
   a.vec = (reinterpret_cast<uintptr_t>(c.out) & 7) == 0 && c.ldo % 4 == 0;
   int m_tiles = 0;
   for (int s = 0; s < t.sec.n; ++s) {
     a.start[s] = s == 0 ? 0 : t.sec.end[s - 1];
     a.end[s] = t.sec.end[s];
+    a.b_start[s] = s == 0 ? 0 : a.b_start[s - 1] + (a.end[s - 1] - a.start[s - 1] + 7) / 8;
     a.first_tile[s] = m_tiles;
     m_tiles += (a.end[s] - a.start[s] + FEATURES - 1) / FEATURES;
     if (a.start[s] % 4) a.vec = 0;
@@ -621,25 +863,32 @@ int launch_tiles(const Call& c) {
   int cs = tiles > SMS ? 1 : power_below((int)(2 * SMS / tiles));
   if (cs > a.kb) cs = power_below(a.kb);
   size_t smem;
-  a.stages = ring_stages<BN>(tiles * cs <= SMS ? SMEM_LIMIT : 113 * 1024, smem);
+  a.stages = ring_stages(tiles * cs <= SMS ? SMEM_LIMIT : HALF_SM, stage_bytes<BN>(), (size_t)BN * RED_PITCH * 4, smem);
   CUtensorMap tw, tx, tb, th;
   int rc = prism_get_tensor_map(c.w, (unsigned long long)c.M, (unsigned long long)c.K, (unsigned long long)c.ldw, FEATURES, &tw);
   if (!rc) rc = prism_get_tensor_map(c.x, (unsigned long long)c.T, (unsigned long long)c.K, (unsigned long long)c.ldx, BN, &tx);
-  if (!rc) rc = prism_make_panel_tensor_map(c.b, (unsigned long long)t.slots * t.panels * c.M, FEATURES, &tb);
-  if (!rc) rc = prism_make_panel_tensor_map(c.h, (unsigned long long)t.tiles * t.capacity * all * c.tile_rows, BN, &th);
+  if (!rc) rc = prism_make_panel_tensor_map(c.b, (unsigned long long)a.no_group, FEATURES / 8, &tb);
+  if (!rc) rc = prism_make_panel_tensor_map(c.h, (unsigned long long)t.tiles * t.capacity * all * c.tile_rows / 8, BN / 8, &th);
   if (rc) return rc;
-  // the launch before is this call's own, which waited for everything older: its early loads are weights
   return (int)prism_launch_clusters(adapter_gemm_kernel<BN, DUAL>, dim3(m_tiles, token_tiles, cs), dim3(TC_THREADS), smem, c.stream, true, cs, tw, tx, tb,
                                     th, a);
 }
 
 template <int BN>
-int launch_both(const Call& c) {
-  const int rc = launch_low<BN>(c);
+int launch_decode(const Call& c) {
+  // Many panels: 16 at a time read the tokens half as often and keep twice the bytes in flight (128 adapters of rank 64, 12288 features).
+  const bool wide = c.terms.capacity * c.terms.panels * c.terms.sec.n > 8 * SMS / 4;
+  const int rc = wide ? launch_low<BN, 2>(c) : launch_low<BN, 1>(c);
   if (rc) return rc;
-  if (c.T > 128 && prism_adapter_pair_fits(c.M, c.act != 0, c.terms, c.out, c.ldo, c.bias))
-    return prism_adapter_pair(c.w, c.x, c.out, c.M, c.T, c.K, c.ldw, c.ldx, c.ldo, c.bias, c.act != 0, c.act, c.terms, c.stream, true);
   return c.act ? launch_tiles<BN, true>(c) : launch_tiles<BN, false>(c);
+}
+
+int launch_prompt(const Call& c) {
+  const int rc = launch_low_prompt(c);
+  if (rc) return rc;
+  if (prism_adapter_pair_fits(c.M, c.act != 0, c.terms, c.out, c.ldo, c.bias))
+    return prism_adapter_pair(c.w, c.x, c.out, c.M, c.T, c.K, c.ldw, c.ldx, c.ldo, c.bias, c.act != 0, c.act, c.terms, c.stream, true);
+  return c.act ? launch_tiles<128, true>(c) : launch_tiles<128, false>(c);
 }
 
 }  // namespace
@@ -664,15 +913,20 @@ PRISM_API int prism_adapter_expand(int f32, const void* base, const void* h, con
                                    int T, int M, int panels, int slots, int sections, const void* ends, int gated, long long ldo, void* stream,
                                    int pdl) {
   if (T < 1 || T > 65535 || M < 1 || panels < 1 || sections < 1 || sections > MAX_SECTIONS || slots < 1 || (gated && (M % 2 || sections != 2))) return -1;
-  ExpandArgs e{(const float*)base, (const float*)h, b, bias, (const int*)adapter, out, T, M, sections * panels * 16, panels, slots, sections, {}, gated, ldo};
-  for (int s = 0; s < sections; ++s) e.end[s] = ((const int*)ends)[s];
+  ExpandArgs e{(const float*)base, (const float*)h, b, bias, (const int*)adapter, out, T, M, sections * panels * 16, panels, slots, sections, 0, {}, {}, gated, ldo};
+  for (int s = 0; s < sections; ++s) {
+    const int start = s ? e.end[s - 1] : 0;
+    e.end[s] = ((const int*)ends)[s];
+    e.shift[s] = e.b_rows - start;
+    e.b_rows += (e.end[s] - start + 7) / 8 * 8;
+  }
   const int features = gated ? M / 2 : M;
   return (int)prism_launch(f32 ? adapter_expand_kernel<float> : adapter_expand_kernel<bf16>, dim3((features + 255) / 256, T), dim3(256), 0,
                            (cudaStream_t)stream, pdl != 0, e);
 }
 
 // bf16 projection (act 0) or gated unit (PRISM_GLU_*) with the adapters of a plan.  lists, counts: of the call's tiles of 256 tokens;
-// h: tiles x capacity x all panels x tile_rows x 16 bf16 of workspace, tile_rows 16, 32, 64, 128 (as many as the tokens need) or 256.
+// b: [slots][panels] panels; h: tiles x capacity x all panels x tile_rows x 16 bf16 of workspace, tile_rows 16, 32, 64, 128 (as many as the tokens need) or 256.
 PRISM_API int prism_adapter_linear(const void* x, const void* w, const void* a, const void* b, const void* scale, const void* index,
                                    const void* lists, const void* counts, const void* bias, void* out, void* h, int T, int M, int K, int slots,
                                    int panels, int sections, const void* ends, int capacity, int tile_rows, int act, long long ldx, long long ldw,
@@ -701,10 +955,12 @@ PRISM_API int prism_adapter_linear(const void* x, const void* w, const void* a, 
   c.terms.sec.n = sections;
   for (int s = 0; s < sections; ++s) {
     c.terms.sec.end[s] = ((const int*)ends)[s];
-    if (c.terms.sec.end[s] <= (s ? c.terms.sec.end[s - 1] : 0)) return -4;
+    const int width = c.terms.sec.end[s] - (s ? c.terms.sec.end[s - 1] : 0);
+    if (width < 1) return -4;
+    c.terms.b_rows += (width + 7) / 8 * 8;
   }
   if (c.terms.sec.end[sections - 1] != M) return -4;
-  if ((long long)slots * panels * M >= 0x7fffffffll || (long long)c.terms.tiles * capacity * panels * sections * tile_rows >= 0x7fffffffll) return -5;
+  if ((long long)slots * panels * c.terms.b_rows >= 0x7fffffffll || (long long)c.terms.tiles * capacity * panels * sections * tile_rows >= 0x7fffffffll) return -5;
   c.bias = bias;
   c.out = out;
   c.ldo = ldo;
@@ -716,10 +972,11 @@ PRISM_API int prism_adapter_linear(const void* x, const void* w, const void* a, 
   c.tile_rows = tile_rows;
   c.stream = (cudaStream_t)stream;
   c.pdl = pdl != 0;
+  if (T > 128) return launch_prompt(c);
   switch (bn) {
-    case 16: return launch_both<16>(c);
-    case 32: return launch_both<32>(c);
-    case 64: return launch_both<64>(c);
-    default: return launch_both<128>(c);
+    case 16: return launch_decode<16>(c);
+    case 32: return launch_decode<32>(c);
+    case 64: return launch_decode<64>(c);
+    default: return launch_decode<128>(c);
   }
 }

@@ -375,14 +375,14 @@ __device__ __forceinline__ uint64_t umma_desc_sw128(uint32_t smem_addr) {
   d |= (uint64_t)2 << 61;            // SWIZZLE_128B
   return d;
 }
-// K-major bf16 tile whose rows are 32 bytes (16 elements, one MMA's worth) with the 32-byte swizzle: 8-row groups are 256 bytes apart.
-__device__ __forceinline__ uint64_t umma_desc_sw32(uint32_t smem_addr) {
+// K-major bf16 panel of 16 columns (one MMA's worth) without swizzle: pieces of 8 rows x 16 bytes, the two of a row group side by side, row
+// groups 256 bytes apart.
+__device__ __forceinline__ uint64_t umma_desc_panel(uint32_t smem_addr) {
   uint64_t d = 0;
   d |= (uint64_t)((smem_addr & 0x3FFFFu) >> 4);
-  d |= (uint64_t)1 << 16;
-  d |= (uint64_t)(256 >> 4) << 32;
+  d |= (uint64_t)(128 >> 4) << 16;   // leading byte offset: the next 8 columns
+  d |= (uint64_t)(256 >> 4) << 32;   // stride byte offset: the next 8 rows
   d |= (uint64_t)1 << 46;
-  d |= (uint64_t)6 << 61;            // SWIZZLE_32B
   return d;
 }
 // MN-major bf16 tile with the 128-byte swizzle: rows are 64 elements along M/N (128 bytes), one
@@ -412,19 +412,21 @@ int prism_get_tensor_map(const void* ptr, unsigned long long rows, unsigned long
 // head_dim read as zeros); see gemm_tcgen05.cu.
 int prism_make_head_tensor_map(const void* ptr, unsigned long long tokens, unsigned heads, unsigned head_dim,
                                unsigned long long ld, unsigned box_rows, CUtensorMap* out);
-// [rows][16] bf16 panels (contiguous rows of 32 bytes), box = box_rows x 16, 32-byte swizzle; not cached.
-int prism_make_panel_tensor_map(const void* ptr, unsigned long long rows, unsigned box_rows, CUtensorMap* out);
+// Panels of 16 ranks in memory as the MMA reads them: groups of 8 rows, each [2][8 rows][8 ranks] bf16 = 256 bytes.  A copy moves box_groups
+// groups; 256-byte rows of the copy engine (as [rows][16] with 32-byte rows, a panel of 128 rows took it some 0.2 us).  Not cached.
+int prism_make_panel_tensor_map(const void* ptr, unsigned long long groups, unsigned box_groups, CUtensorMap* out);
 // Prompt products with low-rank adapters on SM pairs (gemm_pair.cuh), as adapters.cu describes them.
 struct PrismAdapterSections {
   int n;            // sections of the stacked matrix
   int end[8];       // first feature behind each
 };
 struct PrismAdapterTerms {
-  const void* h;            // [tiles of 256 tokens][capacity][panels of all sections][256][16]: a token's low-rank row in its adapter's panels, else zeros
-  const void* b;            // [slots][panels][M][16]
+  const void* h;            // [tiles of 256 tokens][capacity][panels of all sections] panels: a token's low-rank row in its adapter's panels, else zeros
+  const void* b;            // [slots][panels] panels of b_rows rows
   const int* lists;         // [tiles][capacity] slots in use
   const int* counts;        // [tiles]
   int tiles, capacity, panels, slots;
+  int b_rows;               // features of a panel, every section rounded up to 8
   PrismAdapterSections sec;
 };
 bool prism_adapter_pair_fits(int M, int dual, const PrismAdapterTerms& t, const void* out, long long ldo, const void* bias);

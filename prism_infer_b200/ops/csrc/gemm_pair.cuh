@@ -130,7 +130,7 @@ struct PairAdapters {
   const int* lists;
   const int* counts;
   int capacity, panels, all_panels;   // panels of one section, of all sections
-  int b_rows, no_row;                 // rows of one panel of B (features); a row behind all of them, which reads as zeros
+  int b_groups, no_group;             // groups of 8 features in a panel of B; a group behind all of them, which reads as zeros
   int sections;
   int start[8], end[8], first_tile[8];  // feature tiles do not cross sections
 };
@@ -226,13 +226,19 @@ __device__ __forceinline__ void gemm_pair_body(const CUtensorMap& tmX, const CUt
         pair_tma_load_2d(smem + (size_t)s * stage_bytes + A_BYTES, &tmW, cluster_addr(&full[s], 0), kb * 64, row);
       };
       for (int i = 0; i < pre; ++i) load_w(i, kb0 + i, n0);
-      pdl_wait();  // activations come from the previous kernel
+      if (!ADAPTERS) pdl_wait();  // activations come from the previous kernel; with adapters only the low-rank rows do
       for (int tile = pair; tile < num_tiles && ok; tile += pairs) {
         tile_at(tile, m0, n0, kb0, kb1);
-        int extra = 0;
+        int extra = 0, slot = 0, next = 0;   // panels; the slots of the first two adapters, asked for a tile's whole sum ahead
+        const int* list = nullptr;
         if (ADAPTERS) {
           section = section_at(n0);
           extra = panels_of(m0);
+          list = d.lists + (size_t)(m0 / 256) * d.capacity;
+          if (extra > 0) {
+            slot = list[0];
+            next = list[min(1, d.capacity - 1)];
+          }
         }
         for (int kb = kb0; kb < kb1; ++kb) {
           ok = pair_wait(&empty[s], parity, 1);
@@ -244,13 +250,12 @@ __device__ __forceinline__ void gemm_pair_body(const CUtensorMap& tmX, const CUt
           if (++s == stages) s = 0, parity ^= 1, reused = true;
         }
         if (ADAPTERS) {
-          const int per = a.dual ? d.all_panels : d.panels;
-          const int* const list = d.lists + (size_t)(m0 / 256) * d.capacity;
+          pdl_wait();   // the low-rank rows
+          const int of0 = a.dual ? 0 : section * d.panels;
+          const int f = a.dual ? n0 / 2 + (rank ? a.up_row : 0) : n0 + (int)rank * (a.bn / 2);   // first feature of this CTA's half
+          int j = 0, of = of0, rp = 0;   // adapter in the list, panel among those of all sections, and among its section's
           for (int e0 = 0; e0 < extra && ok; e0 += 4) {
             const int n = min(4, extra - e0);
-            int slot[4];   // asked for before the wait
-#pragma unroll
-            for (int i = 0; i < 4; ++i) slot[i] = i < n ? list[(e0 + i) / per] : 0;
             ok = pair_wait(&empty[s], parity, 1);
             if (!ok) break;
             if (rank == 0 && reused) mbar_arrive_cluster_relaxed(cluster_addr(&empty[s], 1));
@@ -260,14 +265,20 @@ __device__ __forceinline__ void gemm_pair_body(const CUtensorMap& tmX, const CUt
 #pragma unroll
             for (int i = 0; i < 4; ++i)
               if (i < n) {
-                const int j = (e0 + i) / per, q = (e0 + i) - j * per;   // the adapter, the panel among those of the tile
-                const int of = a.dual ? q : section * d.panels + q, rp = of % d.panels;
-                pair_tma_load_2d(st + i * 4096, &tmH, bar, 0, ((m0 / 256 * d.capacity + j) * d.all_panels + of) * 256 + (int)rank * 128);
-                int row = (slot[i] * d.panels + rp) * d.b_rows;
-                if (!a.dual) row += n0 + (int)rank * (a.bn / 2);
-                else if (of / d.panels == (int)rank) row += n0 / 2 + (rank ? a.up_row : 0);
-                else row = d.no_row;   // a gate's panel adds nothing to the up half, and the other way round
-                pair_tma_load_2d(st + A_BYTES + i * a.bn * 16, &tmB, bar, 0, row);
+                pair_tma_load_2d(st + i * 4096, &tmH, bar, 0, ((m0 / 256 * d.capacity + j) * d.all_panels + of) * 32 + (int)rank * 16);
+                // a gate's panel adds nothing to the up half (the odd CTA's), and the other way round
+                const bool mine = !a.dual || (of >= d.panels) == (rank != 0);
+                pair_tma_load_2d(st + A_BYTES + i * a.bn * 16, &tmB, bar, 0, mine ? (slot * d.panels + rp) * d.b_groups + f / 8 : d.no_group);
+                ++of;
+                if (++rp == d.panels) {
+                  rp = 0;
+                  if (!a.dual || of == d.all_panels) {
+                    of = of0;
+                    ++j;
+                    slot = next;
+                    next = list[min(j + 1, d.capacity - 1)];
+                  }
+                }
               }
             if (++s == stages) s = 0, parity ^= 1, reused = true;
           }
@@ -287,7 +298,6 @@ __device__ __forceinline__ void gemm_pair_body(const CUtensorMap& tmX, const CUt
       int s = 0, local = 0;
       uint32_t parity = 0;
       bool ok = true;
-      if (ADAPTERS) pdl_wait();   // counts come from the previous kernels
       for (int tile = pair; tile < num_tiles && ok; tile += pairs, ++local) {
         const int buf = local & 1;
         if (local >= 2) {
@@ -317,7 +327,7 @@ __device__ __forceinline__ void gemm_pair_body(const CUtensorMap& tmX, const CUt
             tc_fence_after();
             const uint32_t st = smem_u32(smem + (size_t)s * stage_bytes);
             for (int i = 0; i < min(4, extra - e0); ++i)
-              pair_mma(acc, umma_desc_sw32(st + i * 4096), umma_desc_sw32(st + A_BYTES + i * a.bn * 16), idesc, 1);
+              pair_mma(acc, umma_desc_panel(st + i * 4096), umma_desc_panel(st + A_BYTES + i * a.bn * 16), idesc, 1);
             pair_commit(&empty[s]);
             if (++s == stages) s = 0, parity ^= 1;
           }

@@ -839,12 +839,15 @@ int rounds_of(long long tiles, int places) { return (int)((tiles + places - 1) /
 // Columns of a pair's tile.  A k-block of a tile takes 390 cycles (issue and barriers) or 2.7 per column, whichever is longer
 // (measured over 64 to 256 columns), and the launch as many rounds of tiles as the pairs need: 1616 x 4096 -> 4096 took 44 us with
 // 224 columns (two rounds of a few more columns than half of 256), 47 with 256, 56 with 128.
-int pair_columns(int m_tiles, int columns, bool dual, int* best_rounds = nullptr) {
+// Tiles do not cross sections (n of them, one unless their features have adapters).
+int pair_columns(int m_tiles, int n, const int* columns, bool dual, int* best_rounds = nullptr) {
   const int pairs = sm_count() / 2, step = dual ? 64 : 32;
   int best = 64;
   long long best_cost = 0;
   for (int bn = 64; bn <= 256; bn += step) {
-    const int rounds = rounds_of((long long)m_tiles * ((columns + bn - 1) / bn), pairs);
+    long long tiles = 0;
+    for (int i = 0; i < n; ++i) tiles += (columns[i] + bn - 1) / bn;
+    const int rounds = rounds_of(m_tiles * tiles, pairs);
     const long long cost = (long long)rounds * ((bn < 144 ? 144 : bn) + 8);
     if (best_cost == 0 || cost < best_cost) {
       best = bn, best_cost = cost;
@@ -861,7 +864,7 @@ int pair_columns(int m_tiles, int columns, bool dual, int* best_rounds = nullptr
 int slab_token_tile(int M, int T, int splits) {
   const int m_tiles = (M + BM - 1) / BM, t_tiles = (T + 255) / 256;
   int rounds = 1;
-  const int columns = pair_columns(t_tiles * splits, M, false, &rounds);
+  const int columns = pair_columns(t_tiles * splits, 1, &M, false, &rounds);
   if (M <= 128 || ((T <= 256 || M <= 512) && columns == 64)) return 0;
   if ((long long)m_tiles * ((T + 127) / 128) * splits <= sm_count()) return 128;
   return rounds > 1 && (long long)m_tiles * t_tiles * splits <= sm_count() ? 256 : 0;
@@ -869,7 +872,7 @@ int slab_token_tile(int M, int T, int splits) {
 
 int launch_pair(const void* W, const void* X, int K, long long ldw, long long ldx, int w_rows, PairArgs& a, cudaStream_t stream, bool pdl) {
   a.m_tiles = (a.T + 255) / 256;
-  a.bn = pair_columns(a.m_tiles * a.splits, a.N, a.dual != 0);
+  a.bn = pair_columns(a.m_tiles * a.splits, 1, &a.N, a.dual != 0);
   a.n_tiles = (a.N + a.bn - 1) / a.bn;
   const int stage_bytes = W_TILE_BYTES + a.bn * 64;
   a.stages = (SMEM_LIMIT - 1024 - 512 - PAIR_TURN_BYTES) / stage_bytes;
@@ -912,16 +915,16 @@ int prism_make_head_tensor_map(const void* ptr, unsigned long long tokens, unsig
   return r == CUDA_SUCCESS ? 0 : -102 - (int)r;
 }
 
-int prism_make_panel_tensor_map(const void* ptr, unsigned long long rows, unsigned box_rows, CUtensorMap* out) {
+int prism_make_panel_tensor_map(const void* ptr, unsigned long long groups, unsigned box_groups, CUtensorMap* out) {
   EncodeTiledFn fn = get_encode_fn();
   if (!fn) return -100;
   if (reinterpret_cast<uintptr_t>(ptr) & 15) return -101;
-  cuuint64_t dims[2] = {16, rows};
-  cuuint64_t strides[1] = {32};
-  cuuint32_t box[2] = {16, box_rows};
+  cuuint64_t dims[2] = {128, groups};
+  cuuint64_t strides[1] = {256};
+  cuuint32_t box[2] = {128, box_groups};
   cuuint32_t estr[2] = {1, 1};
   CUresult r = fn(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(ptr), dims, strides, box, estr,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_32B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? 0 : -102 - (int)r;
 }
@@ -958,10 +961,12 @@ int prism_adapter_pair(const void* W, const void* X, void* out, int M, int T, in
   d.capacity = t.capacity;
   d.panels = t.panels;
   d.all_panels = t.panels * t.sec.n;
-  d.b_rows = M;
-  d.no_row = t.slots * t.panels * M;
+  d.b_groups = t.b_rows / 8;
+  d.no_group = t.slots * t.panels * d.b_groups;
   d.sections = t.sec.n;
-  a.bn = pair_columns(a.m_tiles, M, dual != 0);
+  int widths[8];
+  for (int s = 0; s < t.sec.n; ++s) widths[s] = t.sec.end[s] - (s ? t.sec.end[s - 1] : 0);
+  a.bn = pair_columns(a.m_tiles, dual ? 1 : t.sec.n, dual ? &M : widths, dual != 0);
   a.n_tiles = 0;
   for (int s = 0; s < t.sec.n; ++s) {
     d.start[s] = s == 0 ? 0 : t.sec.end[s - 1];
@@ -977,8 +982,8 @@ int prism_adapter_pair(const void* W, const void* X, void* out, int M, int T, in
   CUtensorMap tx, tw, th, tb;
   int rc = get_tensor_map(X, (unsigned long long)T, (unsigned long long)K, (unsigned long long)ldx, 128, &tx);
   if (!rc) rc = get_tensor_map(W, (unsigned long long)M, (unsigned long long)K, (unsigned long long)ldw, (unsigned)(a.bn / 2), &tw);
-  if (!rc) rc = prism_make_panel_tensor_map(t.h, (unsigned long long)t.tiles * t.capacity * d.all_panels * 256, 128, &th);
-  if (!rc) rc = prism_make_panel_tensor_map(t.b, (unsigned long long)t.slots * t.panels * M, (unsigned)(a.bn / 2), &tb);
+  if (!rc) rc = prism_make_panel_tensor_map(t.h, (unsigned long long)t.tiles * t.capacity * d.all_panels * 32, 16, &th);
+  if (!rc) rc = prism_make_panel_tensor_map(t.b, (unsigned long long)d.no_group, (unsigned)(a.bn / 16), &tb);
   if (rc) return rc;
   const cudaError_t e = cudaFuncSetAttribute(gemm_pair_adapter_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_LIMIT);
   if (e != cudaSuccess) return (int)e;
