@@ -218,14 +218,9 @@ def _run(x, w, pool, p, bias, out, act):
 
 def _run_f32(x, w, pool, p, bias, out, act):
     T = x.shape[0]
-    base = torch.empty(T, pool.features, dtype=torch.float32, device=x.device)
-    native.call("prism_gemm_f32", _p(w), _p(x), _p(base), pool.features, T, pool.in_features, _ld(w), _ld(x), pool.features,
-                None, 0, None, None, None, 0.0, _s(), _pdl())
     h = torch.empty(T, pool.low, dtype=torch.float32, device=x.device)
-    native.call("prism_adapter_shrink", 1, _p(x), _p(pool.a), _p(pool.scale), _p(p.adapter), _p(h), T, pool.in_features, pool.low, pool.slots,
-                _ld(x), _s(), _pdl())
-    native.call("prism_adapter_expand", 1, _p(base), _p(h), _p(pool.b), _p(bias), _p(p.adapter), _p(out), T, pool.features, pool.panels,
-                pool.slots, len(pool.sections), pool._ends, act, _ld(out), _s(), _pdl())
+    native.call("prism_adapter_linear_f32", _p(x), _p(w), _p(pool.a), _p(pool.b), _p(pool.scale), _p(p.adapter), _p(bias), _p(out), _p(h), T,
+                pool.features, pool.in_features, pool.slots, pool.panels, len(pool.sections), pool._ends, act, _ld(x), _ld(w), _ld(out), _s(), _pdl())
     return out
 
 

@@ -8,7 +8,6 @@
 #include "common.cuh"
 
 #include <atomic>
-#include <type_traits>
 
 PRISM_DEFINE_TU_STATUS(adapters)
 
@@ -62,84 +61,6 @@ __global__ void __launch_bounds__(PLAN_TILE) adapter_plan_kernel(const int* adap
   if (threadIdx.x == 0) counts[blockIdx.x] = total;
   __syncthreads();
   if (t < T) index[t] = who < 0 ? -1 : before[who >> 5] + __popc(bits[who >> 5] & ((1u << (who & 31)) - 1));
-}
-
-__device__ __forceinline__ float to_float(float v) { return v; }
-__device__ __forceinline__ float to_float(bf16 v) { return __bfloat162float(v); }
-
-struct ShrinkArgs {
-  const void* x;        // [T][ldx]
-  const void* a;        // [slots][low][K]
-  const float* scale;   // [slots]
-  const int* adapter;   // [T]
-  float* h;             // [T][low]
-  int T, K, low, slots;
-  long long ldx;
-};
-
-// h_t = scale A x_t.  One block per token, a warp per row of A.
-template <typename T>
-__global__ void __launch_bounds__(256) adapter_shrink_kernel(const ShrinkArgs a) {
-  const int t = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  pdl_launch_dependents();
-  pdl_wait();
-  const int who = a.adapter[t];
-  if (who < 0 || who >= a.slots) return;
-  const T* const x = (const T*)a.x + (size_t)t * a.ldx;
-  const float scale = a.scale[who];
-  for (int r = warp; r < a.low; r += 8) {
-    const T* const row = (const T*)a.a + ((size_t)who * a.low + r) * a.K;
-    float sum = 0.0f;
-    for (int k = lane; k < a.K; k += 32) sum += to_float(x[k]) * to_float(row[k]);
-    sum = warp_sum(sum);
-    if (lane == 0) a.h[(size_t)t * a.low + r] = sum * scale;
-  }
-}
-
-struct ExpandArgs {
-  const float* base;    // [T][M] W x
-  const float* h;       // [T][low]
-  const void* b;        // [slots][panels][b_rows][16]
-  const void* bias;     // [M] (null: none)
-  const int* adapter;   // [T]
-  void* out;            // [T][ldo]
-  int T, M, low, panels, slots, sections, b_rows;
-  int end[MAX_SECTIONS], shift[MAX_SECTIONS];   // shift: of a section's features in b
-  int gated;            // silu / gelu of the first half times the second half (PRISM_GLU_*), 0: plain
-  long long ldo;
-};
-
-template <typename T>
-__device__ __forceinline__ float adapted(const ExpandArgs& a, int t, int m, int who) {
-  float v = a.base[(size_t)t * a.M + m];
-  if (a.bias != nullptr) v += to_float(((const T*)a.bias)[m]);
-  if (who < 0) return v;
-  int s = 0;
-  while (s + 1 < a.sections && m >= a.end[s]) ++s;
-  const float* const h = a.h + (size_t)t * a.low + s * a.panels * 16;
-  float sum = 0.0f;
-  for (int p = 0; p < a.panels; ++p) {
-    const T* const b = (const T*)a.b + (((size_t)who * a.panels + p) * a.b_rows + m + a.shift[s]) * 16;
-#pragma unroll
-    for (int r = 0; r < 16; ++r) sum += h[p * 16 + r] * to_float(b[r]);
-  }
-  return v + sum;
-}
-
-// y_t = base_t + bias + B h_t, through the gated unit if asked for; a thread per feature.
-template <typename T>
-__global__ void __launch_bounds__(256) adapter_expand_kernel(const ExpandArgs a) {
-  const int m = blockIdx.x * 256 + threadIdx.x, t = blockIdx.y, out_features = a.gated ? a.M / 2 : a.M;
-  pdl_launch_dependents();
-  pdl_wait();
-  if (m >= out_features) return;
-  int who = a.adapter[t];
-  if (who >= a.slots) who = -1;
-  float v = adapted<T>(a, t, m, who);
-  if (a.gated) v = glu(v, adapted<T>(a, t, m + a.M / 2, who), a.gated);
-  T* const out = (T*)a.out + (size_t)t * a.ldo + m;
-  if constexpr (std::is_same<T, float>::value) *out = v;
-  else *out = __float2bfloat16_rn(v);
 }
 
 // ------------------------------------------------------------------------------------------------------------------------------------
@@ -733,6 +654,192 @@ adapter_gemm_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_consta
   }
 }
 
+// ------------------------------------------------------------------------------------------------------------------------------------
+// fp32: true 32-bit multiply-adds.  The low-rank rows first, a block per token; then the projection in tiles of 64 features x TN tokens, a
+// thread summing 4 x NT of them, whose epilogue adds each token's low-rank term.  Clusters split K where the tiles are few.
+// Sums run over 128 products in one accumulator, which is then added to another: a plain chain over K = 7064 was off by five times as much
+// (1.1e-6 of the outputs' scale against 2e-7).
+// ------------------------------------------------------------------------------------------------------------------------------------
+struct LowF32Args {
+  const float* x;       // [T][ldx]
+  const float* a;       // [slots][low][K]
+  const float* scale;   // [slots]
+  const int* adapter;   // [T]
+  float* h;             // [T][low]; rows of tokens without an adapter are not written
+  int K, low, slots, vec;
+  long long ldx;
+};
+
+// Four consecutive values, zeros behind the end.
+__device__ __forceinline__ float4 load4(const float* p, int k, int K, bool vec) {
+  if (vec && k + 4 <= K) return *reinterpret_cast<const float4*>(p + k);
+  return make_float4(k < K ? p[k] : 0.0f, k + 1 < K ? p[k + 1] : 0.0f, k + 2 < K ? p[k + 2] : 0.0f, k + 3 < K ? p[k + 3] : 0.0f);
+}
+
+// A warp per two rows of A, whose sums it keeps in four parts per lane.
+__global__ void __launch_bounds__(256) adapter_low_f32_kernel(const LowF32Args a) {
+  const int t = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  pdl_wait();
+  pdl_launch_dependents();   // the projection reads h last
+  const int who = a.adapter[t];
+  if (who < 0 || who >= a.slots) return;
+  const float* const x = a.x + (size_t)t * a.ldx;
+  const float scale = a.scale[who];
+  for (int r = (blockIdx.y * 8 + warp) * 2; r < a.low; r += gridDim.y * 16) {
+    const float* const row = a.a + ((size_t)who * a.low + r) * a.K;
+    float4 s0 = make_float4(0, 0, 0, 0), s1 = s0;
+#pragma unroll 4
+    for (int k = lane * 4; k < a.K; k += 128) {
+      const float4 v = load4(x, k, a.K, a.vec), p = load4(row, k, a.K, a.vec), q = load4(row + a.K, k, a.K, a.vec);
+      s0 = make_float4(fmaf(v.x, p.x, s0.x), fmaf(v.y, p.y, s0.y), fmaf(v.z, p.z, s0.z), fmaf(v.w, p.w, s0.w));
+      s1 = make_float4(fmaf(v.x, q.x, s1.x), fmaf(v.y, q.y, s1.y), fmaf(v.z, q.z, s1.z), fmaf(v.w, q.w, s1.w));
+    }
+    const float u = warp_sum((s0.x + s0.y) + (s0.z + s0.w)), w = warp_sum((s1.x + s1.y) + (s1.z + s1.w));
+    if (lane < 2) a.h[(size_t)t * a.low + r + lane] = (lane ? w : u) * scale;
+  }
+}
+
+struct TileF32Args {
+  const float* x;       // [T][ldx]
+  const float* w;       // [M][ldw]
+  const float* b;       // [slots][panels][b_rows][16]
+  const float* h;       // [T][low]
+  const float* bias;    // [M] (null: none)
+  const int* adapter;   // [T]
+  float* out;           // [T][ldo]
+  int T, M, K, low, panels, slots, b_rows, vec, act;
+  long long ldx, ldw, ldo;
+  int sections;
+  int end[MAX_SECTIONS], shift[MAX_SECTIONS];   // shift: of a section's features in b
+};
+
+__device__ __forceinline__ float glu_f32(float z, float u, int act) {
+  return (act == PRISM_GLU_GELU_TANH ? 0.5f * z * (1.0f + tanhf(0.7978845608028654f * (z + 0.044715f * z * z * z))) : z / (1.0f + expf(-z))) * u;
+}
+
+// Low-rank term of feature m for the token whose row of h is given.
+__device__ __forceinline__ float low_term(const TileF32Args& a, const float* h, int who, int m) {
+  int s = 0;
+  while (s + 1 < a.sections && m >= a.end[s]) ++s;
+  h += s * a.panels * 16;
+  float sum = 0.0f;
+  for (int p = 0; p < a.panels; ++p) {
+    const float4* const b = reinterpret_cast<const float4*>(a.b + (((size_t)who * a.panels + p) * a.b_rows + m + a.shift[s]) * 16);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float4 v = b[e], g = *reinterpret_cast<const float4*>(h + p * 16 + e * 4);
+      sum += (v.x * g.x + v.y * g.y) + (v.z * g.z + v.w * g.w);
+    }
+  }
+  return sum;
+}
+
+constexpr int F32_THREADS = 128, F32_K = 32, F32_FOLD = 4;   // F32_FOLD chunks of F32_K products per accumulator
+
+template <int NT, bool DUAL>
+__global__ void __launch_bounds__(F32_THREADS, 4) adapter_gemm_f32_kernel(const TileF32Args a) {
+  constexpr int TN = 8 * NT, WP = 68, XP = TN + 4, LOADS = TN * F32_K / 4 / F32_THREADS, QUADS = DUAL ? 8 : 16, RED = 68;
+  __shared__ __align__(16) float ws[2][F32_K][WP];
+  __shared__ __align__(16) float xs[2][F32_K][XP];
+  static_assert(TN * RED <= 2 * F32_K * WP, "the sums take the weights' place");
+  float* const red = &ws[0][0][0];
+  const int cs = gridDim.z, z = blockIdx.z, tid = threadIdx.x;
+  const int f0 = blockIdx.x * (DUAL ? 32 : 64), t0 = blockIdx.y * TN, half = a.M / 2;
+  const int chunks = (a.K + F32_K - 1) / F32_K, c0 = part_begin(chunks, z, cs), c1 = part_begin(chunks, z + 1, cs);
+  // row i of the weight tile; a row outside the matrix reads as zeros
+  auto w_row = [&](int i) { return DUAL ? (i < 32 ? (f0 + i < half ? f0 + i : -1) : (f0 + i - 32 < half ? half + f0 + i - 32 : -1)) : (f0 + i < a.M ? f0 + i : -1); };
+  float4 wr[4], xr[LOADS];
+  auto fetch = [&](int chunk) {
+    const int k = chunk * F32_K + (tid & 7) * 4;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = w_row((tid >> 3) + i * 16);
+      wr[i] = r < 0 ? make_float4(0, 0, 0, 0) : load4(a.w + (size_t)r * a.ldw, k, a.K, a.vec);
+    }
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const int t = t0 + (tid >> 3) + i * 16;
+      xr[i] = t < a.T ? load4(a.x + (size_t)t * a.ldx, k, a.K, a.vec) : make_float4(0, 0, 0, 0);
+    }
+  };
+  auto keep = [&](int buf) {   // turned: k by k
+    const int k = (tid & 7) * 4;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = (tid >> 3) + i * 16;
+      ws[buf][k][r] = wr[i].x, ws[buf][k + 1][r] = wr[i].y, ws[buf][k + 2][r] = wr[i].z, ws[buf][k + 3][r] = wr[i].w;
+    }
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const int r = (tid >> 3) + i * 16;
+      xs[buf][k][r] = xr[i].x, xs[buf][k + 1][r] = xr[i].y, xs[buf][k + 2][r] = xr[i].z, xs[buf][k + 3][r] = xr[i].w;
+    }
+  };
+  const int fx = (tid & 15) * 4, tx = (tid >> 4) * NT;   // this thread's 4 features and NT tokens
+  float acc[NT][4] = {}, total[NT][4] = {};
+  pdl_launch_dependents();
+  fetch(c0);
+  keep(0);
+  __syncthreads();
+  for (int c = c0; c < c1; ++c) {
+    const int buf = (c - c0) & 1;
+    if (c + 1 < c1) fetch(c + 1);
+#pragma unroll
+    for (int k = 0; k < F32_K; ++k) {
+      const float4 w = *reinterpret_cast<const float4*>(&ws[buf][k][fx]);
+      float x[NT];
+#pragma unroll
+      for (int i = 0; i < NT; i += 2) *reinterpret_cast<float2*>(&x[i]) = *reinterpret_cast<const float2*>(&xs[buf][k][tx + i]);
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+        acc[i][0] = fmaf(x[i], w.x, acc[i][0]);
+        acc[i][1] = fmaf(x[i], w.y, acc[i][1]);
+        acc[i][2] = fmaf(x[i], w.z, acc[i][2]);
+        acc[i][3] = fmaf(x[i], w.w, acc[i][3]);
+      }
+    }
+    if ((c - c0) % F32_FOLD == F32_FOLD - 1 || c + 1 == c1) {
+#pragma unroll
+      for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) total[i][e] += acc[i][e], acc[i][e] = 0.0f;
+    }
+    if (c + 1 < c1) keep(buf ^ 1);
+    __syncthreads();
+  }
+#pragma unroll
+  for (int i = 0; i < NT; ++i) *reinterpret_cast<float4*>(&red[(tx + i) * RED + fx]) = make_float4(total[i][0], total[i][1], total[i][2], total[i][3]);
+  pdl_wait();   // the low-rank rows
+  cluster_sync_all();
+  const int items = min(TN, a.T - t0) * QUADS;
+  for (int i = part_begin(items, z, cs) + tid; i < part_begin(items, z + 1, cs); i += F32_THREADS) {
+    const int c = i / QUADS, f = f0 + (i % QUADS) * 4, n = min(4, (DUAL ? half : a.M) - f);
+    if (n <= 0) continue;
+    const int who_raw = a.adapter[t0 + c], who = who_raw < a.slots ? who_raw : -1;
+    const float* const h = a.h + (size_t)(t0 + c) * a.low;
+    const float4 v = cluster_sum4(red + c * RED + (i % QUADS) * 4, cs);
+    float y[4] = {v.x, v.y, v.z, v.w};
+    float u[4] = {};
+    if (DUAL) {
+      const float4 r = cluster_sum4(red + c * RED + 32 + (i % QUADS) * 4, cs);
+      u[0] = r.x, u[1] = r.y, u[2] = r.z, u[3] = r.w;
+    }
+    float* const dst = a.out + (size_t)(t0 + c) * a.ldo + f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (e >= n) break;
+      if (a.bias != nullptr) y[e] += a.bias[f + e];
+      if (who >= 0) y[e] += low_term(a, h, who, f + e);
+      if (DUAL) {
+        if (who >= 0) u[e] += low_term(a, h, who, half + f + e);
+        y[e] = glu_f32(y[e], u[e], a.act);
+      }
+      dst[e] = y[e];
+    }
+  }
+  cluster_sync_all();   // nobody leaves while a peer may read its sums
+}
+
 constexpr int SMS = 148;
 constexpr int SMEM_LIMIT = 232448 - 2048;   // 227 KB, 2 KB of it for static arrays
 
@@ -760,10 +867,6 @@ int ring_stages(int budget, int stage, size_t red, size_t& smem) {
   return stages;
 }
 
-int power_below(int n) {   // the largest of 1, 2, 4, 8 that is not above n
-  return n >= 8 ? 8 : n >= 4 ? 4 : n >= 2 ? 2 : 1;
-}
-
 struct Call {
   const void *x, *w;
   long long ldx, ldw;
@@ -780,7 +883,46 @@ struct Call {
   bool pdl;
 };
 
-constexpr int HALF_SM = 112 * 1024;   // two such blocks share an SM: the projection's first loads overlap the low-rank rows
+constexpr int HALF_SM = 112 * 1024 + 512;   // two such blocks share an SM: the projection streams weights beside the low-rank rows
+
+// The largest cluster of 8, 4 or 2 blocks along z, at most `most`, of which n fit the device at once; 1 if none does.  More clusters than fit
+// take a second round: 16 clusters of 8 blocks with an SM each took 22 us, 13 of them 11.6.  The count is asked for with an empty kernel: for
+// kernels that allocate tensor memory the runtime counts one block per SM, but two run there where shared memory and columns allow it (256
+// blocks of the projection 12288 -> 4096 38 us, 128 of them 48).
+__global__ void __launch_bounds__(TC_THREADS) placeholder_kernel() {}
+struct ClusterTable {
+  std::atomic<int> known[16][4];   // per device: clusters that fit with one amount of shared memory, plus one
+};
+int cluster_size(ClusterTable& table, long long n, int most, size_t smem) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 1;
+  for (int k = 3; k > 0; --k) {
+    const int cs = 1 << k;
+    if (cs > most) continue;
+    std::atomic<int>* const slot = dev < 16 ? &table.known[dev][k] : nullptr;
+    int fit = slot ? slot->load(std::memory_order_relaxed) - 1 : -1;
+    if (fit < 0) {
+      static std::atomic<unsigned long long> devices{0};
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3(1, 1, cs);
+      cfg.blockDim = dim3(TC_THREADS);
+      cfg.dynamicSmemBytes = smem;
+      cudaLaunchAttribute attr[1];
+      attr[0].id = cudaLaunchAttributeClusterDimension;
+      attr[0].val.clusterDim.x = attr[0].val.clusterDim.y = 1;
+      attr[0].val.clusterDim.z = cs;
+      cfg.attrs = attr;
+      cfg.numAttrs = 1;
+      if (allow_smem(placeholder_kernel, devices) != cudaSuccess || cudaOccupancyMaxActiveClusters(&fit, placeholder_kernel, &cfg) != cudaSuccess) {
+        (void)cudaGetLastError();
+        fit = 0;
+      }
+      if (slot) slot->store(fit + 1, std::memory_order_relaxed);
+    }
+    if (n <= fit) return cs;
+  }
+  return 1;
+}
 
 LowArgs low_args(const Call& c) {
   return LowArgs{c.terms.lists, c.terms.counts, c.index, c.scale, (bf16*)c.h, c.T, (c.K + 63) / 64, c.terms.capacity, c.terms.panels * c.terms.sec.n,
@@ -790,15 +932,15 @@ LowArgs low_args(const Call& c) {
 template <int BN, int G>
 int launch_low(const Call& c) {
   static std::atomic<unsigned long long> devices{0};
+  static ClusterTable table;
   cudaError_t e = allow_smem(adapter_low_kernel<BN, G>, devices);
   if (e != cudaSuccess) return (int)e;
   LowArgs a = low_args(c);
   const int most = (a.capacity * a.all_panels + G * 8 - 1) / (G * 8);   // a step may bring as many adapters as tokens
-  int cs = power_below(SMS / (most > SMS ? SMS : most));
-  if (cs > a.kb) cs = power_below(a.kb);
-  const int gx = SMS / cs < most ? SMS / cs : most;
   size_t smem;
   a.stages = ring_stages(G == 1 ? HALF_SM : SMEM_LIMIT, G * W_BYTES + BN * 128, (size_t)BN * (G * 128 + 4) * 4, smem);
+  const int cs = most > SMS ? 1 : cluster_size(table, most, a.kb < SMS / most ? a.kb : SMS / most, smem);
+  const int gx = SMS / cs < most ? SMS / cs : most;
   CUtensorMap ta, tx;
   int rc = prism_get_tensor_map(c.a, (unsigned long long)c.terms.slots * a.all_panels * 16, (unsigned long long)c.K, (unsigned long long)c.K, 16, &ta);
   if (!rc) rc = prism_get_tensor_map(c.x, (unsigned long long)c.T, (unsigned long long)c.K, (unsigned long long)c.ldx, BN, &tx);
@@ -808,14 +950,14 @@ int launch_low(const Call& c) {
 
 int launch_low_prompt(const Call& c) {
   static std::atomic<unsigned long long> devices{0};
+  static ClusterTable table;
   cudaError_t e = allow_smem(adapter_low_prompt_kernel, devices);
   if (e != cudaSuccess) return (int)e;
   LowArgs a = low_args(c);
   const int tiles = (c.T + 127) / 128;
-  int cs = power_below(SMS / (tiles > SMS ? SMS : tiles));
-  if (cs > a.kb) cs = power_below(a.kb);
   size_t smem;
   a.stages = ring_stages(SMEM_LIMIT, W_BYTES + 16 * 2048, (size_t)16 * 128 * 20 * 4, smem);
+  const int cs = cluster_size(table, tiles, a.kb, smem);
   CUtensorMap ta, tx;
   int rc = prism_get_tensor_map(c.a, (unsigned long long)c.terms.slots * a.all_panels * 16, (unsigned long long)c.K, (unsigned long long)c.K, 16, &ta);
   if (!rc) rc = prism_get_tensor_map(c.x, (unsigned long long)c.T, (unsigned long long)c.K, (unsigned long long)c.ldx, 128, &tx);
@@ -826,6 +968,7 @@ int launch_low_prompt(const Call& c) {
 template <int BN, bool DUAL>
 int launch_tiles(const Call& c) {
   static std::atomic<unsigned long long> devices{0};
+  static ClusterTable table;
   cudaError_t e = allow_smem(adapter_gemm_kernel<BN, DUAL>, devices);
   if (e != cudaSuccess) return (int)e;
   constexpr int FEATURES = DUAL ? 64 : 128;
@@ -860,10 +1003,9 @@ int launch_tiles(const Call& c) {
   }
   if (DUAL) m_tiles = (c.M / 2 + FEATURES - 1) / FEATURES;
   const long long tiles = (long long)m_tiles * token_tiles;
-  int cs = tiles > SMS ? 1 : power_below((int)(2 * SMS / tiles));
-  if (cs > a.kb) cs = power_below(a.kb);
   size_t smem;
-  a.stages = ring_stages(tiles * cs <= SMS ? SMEM_LIMIT : HALF_SM, stage_bytes<BN>(), (size_t)BN * RED_PITCH * 4, smem);
+  a.stages = ring_stages(HALF_SM, stage_bytes<BN>(), (size_t)BN * RED_PITCH * 4, smem);
+  const int cs = tiles > 2 * SMS ? 1 : cluster_size(table, tiles, a.kb, smem);
   CUtensorMap tw, tx, tb, th;
   int rc = prism_get_tensor_map(c.w, (unsigned long long)c.M, (unsigned long long)c.K, (unsigned long long)c.ldw, FEATURES, &tw);
   if (!rc) rc = prism_get_tensor_map(c.x, (unsigned long long)c.T, (unsigned long long)c.K, (unsigned long long)c.ldx, BN, &tx);
@@ -902,27 +1044,42 @@ PRISM_API int prism_adapter_plan(const void* adapter, int T, int slots, int capa
                            (const int*)adapter, T, slots, capacity, (int*)index, (int*)lists, (int*)counts);
 }
 
-PRISM_API int prism_adapter_shrink(int f32, const void* x, const void* a, const void* scale, const void* adapter, void* h, int T, int K, int low,
-                                   int slots, long long ldx, void* stream, int pdl) {
-  if (T < 1 || K < 1 || low < 16 || low % 16 || slots < 1) return -1;
-  ShrinkArgs s{x, a, (const float*)scale, (const int*)adapter, (float*)h, T, K, low, slots, ldx};
-  return (int)prism_launch(f32 ? adapter_shrink_kernel<float> : adapter_shrink_kernel<bf16>, dim3(T), dim3(256), 0, (cudaStream_t)stream, pdl != 0, s);
+namespace {
+
+template <int NT, bool DUAL>
+int launch_f32(const TileF32Args& a, cudaStream_t stream) {
+  static ClusterTable table;
+  const long long tiles = (long long)((DUAL ? a.M / 2 + 31 : a.M + 63) / (DUAL ? 32 : 64)) * ((a.T + 8 * NT - 1) / (8 * NT));
+  const int chunks = (a.K + F32_K - 1) / F32_K;
+  const int cs = cluster_size(table, tiles, chunks / F32_FOLD, 56 * 1024);   // four blocks per SM, at least 128 products each
+  const dim3 grid((unsigned)((DUAL ? a.M / 2 + 31 : a.M + 63) / (DUAL ? 32 : 64)), (unsigned)((a.T + 8 * NT - 1) / (8 * NT)), cs);
+  return (int)prism_launch_clusters(adapter_gemm_f32_kernel<NT, DUAL>, grid, dim3(F32_THREADS), 0, stream, true, cs, a);
 }
 
-PRISM_API int prism_adapter_expand(int f32, const void* base, const void* h, const void* b, const void* bias, const void* adapter, void* out,
-                                   int T, int M, int panels, int slots, int sections, const void* ends, int gated, long long ldo, void* stream,
-                                   int pdl) {
-  if (T < 1 || T > 65535 || M < 1 || panels < 1 || sections < 1 || sections > MAX_SECTIONS || slots < 1 || (gated && (M % 2 || sections != 2))) return -1;
-  ExpandArgs e{(const float*)base, (const float*)h, b, bias, (const int*)adapter, out, T, M, sections * panels * 16, panels, slots, sections, 0, {}, {}, gated, ldo};
+}  // namespace
+
+// The same in 32 bits; b: [slots][panels][rows][16], h: T x low floats of workspace.
+PRISM_API int prism_adapter_linear_f32(const void* x, const void* w, const void* a, const void* b, const void* scale, const void* adapter,
+                                       const void* bias, void* out, void* h, int T, int M, int K, int slots, int panels, int sections, const void* ends,
+                                       int act, long long ldx, long long ldw, long long ldo, void* stream, int pdl) {
+  if (T < 1 || T > 65535 * 16 || M < 1 || K < 1 || slots < 1 || panels < 1 || sections < 1 || sections > MAX_SECTIONS) return -1;
+  if (act && (M % 2 || sections != 2 || bias != nullptr)) return -2;
+  const bool vec = (((uintptr_t)x | (uintptr_t)w | (uintptr_t)a) & 15) == 0 && K % 4 == 0 && ldx % 4 == 0 && ldw % 4 == 0;
+  const int low = sections * panels * 16;
+  LowF32Args l{(const float*)x, (const float*)a, (const float*)scale, (const int*)adapter, (float*)h, K, low, slots, vec, ldx};
+  // few tokens: a block per 16 rows
+  const cudaError_t e = prism_launch(adapter_low_f32_kernel, dim3(T, T < 148 ? (low + 15) / 16 : 1), dim3(256), 0, (cudaStream_t)stream, pdl != 0, l);
+  if (e != cudaSuccess) return (int)e;
+  TileF32Args t{(const float*)x, (const float*)w, (const float*)b, (const float*)h, (const float*)bias, (const int*)adapter, (float*)out,
+                T, M, K, low, panels, slots, 0, vec, act, ldx, ldw, ldo, sections, {}, {}};
   for (int s = 0; s < sections; ++s) {
-    const int start = s ? e.end[s - 1] : 0;
-    e.end[s] = ((const int*)ends)[s];
-    e.shift[s] = e.b_rows - start;
-    e.b_rows += (e.end[s] - start + 7) / 8 * 8;
+    const int start = s ? t.end[s - 1] : 0;
+    t.end[s] = ((const int*)ends)[s];
+    t.shift[s] = t.b_rows - start;
+    t.b_rows += (t.end[s] - start + 7) / 8 * 8;
   }
-  const int features = gated ? M / 2 : M;
-  return (int)prism_launch(f32 ? adapter_expand_kernel<float> : adapter_expand_kernel<bf16>, dim3((features + 255) / 256, T), dim3(256), 0,
-                           (cudaStream_t)stream, pdl != 0, e);
+  if (T <= 16) return act ? launch_f32<2, true>(t, (cudaStream_t)stream) : launch_f32<2, false>(t, (cudaStream_t)stream);
+  return act ? launch_f32<8, true>(t, (cudaStream_t)stream) : launch_f32<8, false>(t, (cudaStream_t)stream);
 }
 
 // bf16 projection (act 0) or gated unit (PRISM_GLU_*) with the adapters of a plan.  lists, counts: of the call's tiles of 256 tokens;

@@ -79,8 +79,7 @@ _SIGNATURES = {
     "prism_kv_compact": "pliplppppiiiip",
     "prism_step_maps": "pppppp" "iiiii" "ppppppppp" "pi",
     "prism_adapter_plan": "piiippppi",
-    "prism_adapter_shrink": "ippppp" "iiiilpi",
-    "prism_adapter_expand": "ipppppp" "iiiiipilpi",
+    "prism_adapter_linear_f32": "ppppppppp" "iiiiii" "pilllpi",
     "prism_adapter_linear": "ppppp" "pppp" "pp" "iiiiii" "piii" "lllpi",
     "prism_sample": "pllipppiilupppipi",
     "prism_merge_candidates": "pppiipi",
