@@ -143,8 +143,8 @@ def plan(adapter: torch.Tensor, slots: int) -> AdapterPlan:
             index[i * TILE_TOKENS:(i + 1) * TILE_TOKENS] = torch.where(who >= 0, torch.searchsorted(used, who).int(), -1)
         return AdapterPlan(adapter, slots, index, lists, counts)
     check_device(adapter)
-    index, _, lists, _, counts = torch.empty(T + -T % 4 + tiles * capacity + -(tiles * capacity) % 4 + tiles, dtype=torch.int32, device=adapter.device).split(
-        (T, -T % 4, tiles * capacity, -(tiles * capacity) % 4, tiles))
+    index, lists, counts = torch.split_with_sizes(torch.empty(T + tiles * capacity + tiles, dtype=torch.int32, device=adapter.device),
+                                                  (T, tiles * capacity, tiles))
     if T:
         native.call("prism_adapter_plan", _p(adapter), T, slots, capacity, _p(index), _p(lists), _p(counts), _s(), _pdl())
     return AdapterPlan(adapter, slots, index, lists.view(tiles, capacity), counts)

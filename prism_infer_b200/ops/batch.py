@@ -78,12 +78,11 @@ def step_maps(pages: torch.Tensor, cached: torch.Tensor, fresh: torch.Tensor, *,
     if not cached.is_cuda:
         return _step_maps_cpu(pages, cached, fresh, page, tokens, width, page_offsets, shift, adapter)
     check_device(cached)
-    # one allocation per type, its parts on 16-byte boundaries
-    sizes = []
-    for n in (S * width, 3 * tokens, tokens, tokens if adapter is not None else 0, S + 1, S + 1, S):
-        sizes += [n, -n % 4]
-    tables, _, positions, _, seq, _, who, _, cu_q, _, cu_kv, _, kv, _ = torch.empty(sum(sizes), dtype=torch.int32, device=device).split(sizes)
-    slots, _, sample = torch.empty(tokens + tokens % 2 + S, dtype=torch.int64, device=device).split((tokens, tokens % 2, S))
+    # one allocation per type
+    tables, positions, seq, who, cu_q, cu_kv, kv = torch.split_with_sizes(
+        torch.empty(S * width + 5 * tokens + 3 * S + 2, dtype=torch.int32, device=device),
+        (S * width, 3 * tokens, tokens, tokens, S + 1, S + 1, S))
+    slots, sample = torch.split_with_sizes(torch.empty(tokens + S, dtype=torch.int64, device=device), (tokens, S))
     native.call("prism_step_maps", _p(pages), _p(page_offsets), _p(cached), _p(fresh), _p(shift), _p(adapter), S, tokens, width, page,
                 pages.shape[0], _p(tables), _p(slots), _p(positions), _p(seq), _p(who) if adapter is not None else None, _p(cu_q), _p(cu_kv),
                 _p(kv), _p(sample), _s(), _pdl())

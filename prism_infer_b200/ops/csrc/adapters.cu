@@ -193,15 +193,18 @@ adapter_low_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
   __shared__ int who[BN];
   __shared__ float scale[BN];
 
-  if (threadIdx.x == 0) {
+  const int kb0 = part_begin(a.kb, blockIdx.z, gridDim.z), kb1 = part_begin(a.kb, blockIdx.z + 1, gridDim.z);
+  // the first tokens are under way before the list of adapters is read; their bytes are announced with those of the factors
+  const int pre = (int)blockIdx.x * G * 8 < panels ? min(stages, kb1 - kb0) : 0;
+  if (warp == 0 && elect_one()) {
     for (int s = 0; s < stages; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
     mbar_init(acc_full, 1);
     fence_barrier_init();
+    for (int i = 0; i < pre; ++i) tma_load_2d(smem + (size_t)i * STAGE + X_AT, &tmX, &full[i], (kb0 + i) * 64, 0);
     tma_prefetch_desc(&tmA);
-    tma_prefetch_desc(&tmX);
   }
   if (warp == 1) {
     tmem_alloc(tmem_slot, TMEM_COLS);
@@ -213,7 +216,6 @@ adapter_low_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  const int kb0 = part_begin(a.kb, blockIdx.z, gridDim.z), kb1 = part_begin(a.kb, blockIdx.z + 1, gridDim.z);
   int s = 0, round = 0;   // ring stage; passes done
   uint32_t parity = 0;    // of the full barriers (MMA); the producer waits for the phase before
   bool ok = true;         // this thread's role goes on; after a wait that ran out it only keeps step with the cluster
@@ -232,7 +234,7 @@ adapter_low_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
           if (!ok) break;
           uint8_t* const st = smem + (size_t)s * STAGE;
           mbar_expect_tx(&full[s], np * 2048 + BN * 128);
-          tma_load_2d(st + X_AT, &tmX, &full[s], kb * 64, 0);
+          if (round > 0 || kb - kb0 >= pre) tma_load_2d(st + X_AT, &tmX, &full[s], kb * 64, 0);
 #pragma unroll
           for (int i = 0; i < G * 8; ++i)
             if (i < np) tma_load_2d(st + i * 2048, &tmA, &full[s], kb * 64, row[i]);
@@ -318,7 +320,8 @@ adapter_low_prompt_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_
   __shared__ int n_active;
   for (int j = threadIdx.x; j < count; j += TC_THREADS) place[j] = -1;
 
-  if (threadIdx.x == 0) {
+  const int kb0 = part_begin(a.kb, blockIdx.z, gridDim.z), kb1 = part_begin(a.kb, blockIdx.z + 1, gridDim.z);
+  if (warp == 0 && elect_one()) {
     for (int s = 0; s < stages; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
@@ -366,7 +369,6 @@ adapter_low_prompt_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_
                                     in_panel(token0 - tile * PLAN_TILE + blockIdx.z * share + (i >> 1) % share, i & 1)) = make_uint4(0, 0, 0, 0);
   }
 
-  const int kb0 = part_begin(a.kb, blockIdx.z, gridDim.z), kb1 = part_begin(a.kb, blockIdx.z + 1, gridDim.z);
   int s = 0, round = 0;
   uint32_t parity = 0;
   bool ok = true;
@@ -762,16 +764,18 @@ __global__ void __launch_bounds__(F32_THREADS, 4) adapter_gemm_f32_kernel(const 
       xr[i] = t < a.T ? load4(a.x + (size_t)t * a.ldx, k, a.K, a.vec) : make_float4(0, 0, 0, 0);
     }
   };
-  auto keep = [&](int buf) {   // turned: k by k
+  // Turned: k by k.  Rows change places with k / 4, which spreads the stores over the banks (without, 1.6 million conflicts in 0.54 million
+  // stores for 100 tokens, 2048 -> 2048).
+  auto keep = [&](int buf) {
     const int k = (tid & 7) * 4;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int r = (tid >> 3) + i * 16;
+      const int r = ((tid >> 3) + i * 16) ^ k;
       ws[buf][k][r] = wr[i].x, ws[buf][k + 1][r] = wr[i].y, ws[buf][k + 2][r] = wr[i].z, ws[buf][k + 3][r] = wr[i].w;
     }
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
-      const int r = (tid >> 3) + i * 16;
+      const int r = ((tid >> 3) + i * 16) ^ (k & (TN - 1));
       xs[buf][k][r] = xr[i].x, xs[buf][k + 1][r] = xr[i].y, xs[buf][k + 2][r] = xr[i].z, xs[buf][k + 3][r] = xr[i].w;
     }
   };
@@ -786,10 +790,10 @@ __global__ void __launch_bounds__(F32_THREADS, 4) adapter_gemm_f32_kernel(const 
     if (c + 1 < c1) fetch(c + 1);
 #pragma unroll
     for (int k = 0; k < F32_K; ++k) {
-      const float4 w = *reinterpret_cast<const float4*>(&ws[buf][k][fx]);
+      const float4 w = *reinterpret_cast<const float4*>(&ws[buf][k][fx ^ (k & ~3)]);
       float x[NT];
 #pragma unroll
-      for (int i = 0; i < NT; i += 2) *reinterpret_cast<float2*>(&x[i]) = *reinterpret_cast<const float2*>(&xs[buf][k][tx + i]);
+      for (int i = 0; i < NT; i += 2) *reinterpret_cast<float2*>(&x[i]) = *reinterpret_cast<const float2*>(&xs[buf][k][(tx + i) ^ (k & ~3 & (TN - 1))]);
 #pragma unroll
       for (int i = 0; i < NT; ++i) {
         acc[i][0] = fmaf(x[i], w.x, acc[i][0]);
@@ -957,7 +961,9 @@ int launch_low_prompt(const Call& c) {
   const int tiles = (c.T + 127) / 128;
   size_t smem;
   a.stages = ring_stages(SMEM_LIMIT, W_BYTES + 16 * 2048, (size_t)16 * 128 * 20 * 4, smem);
-  const int cs = cluster_size(table, tiles, a.kb, smem);
+  // Half the SMs at most: the projection's pairs of SMs that walk one tile more than the others are its first blocks and start on the other
+  // half at once, the rest have as much time for the low-rank rows as a tile takes.
+  const int cs = 2 * tiles > SMS ? 1 : cluster_size(table, tiles, a.kb < SMS / 2 / tiles ? a.kb : SMS / 2 / tiles, smem);
   CUtensorMap ta, tx;
   int rc = prism_get_tensor_map(c.a, (unsigned long long)c.terms.slots * a.all_panels * 16, (unsigned long long)c.K, (unsigned long long)c.K, 16, &ta);
   if (!rc) rc = prism_get_tensor_map(c.x, (unsigned long long)c.T, (unsigned long long)c.K, (unsigned long long)c.ldx, 128, &tx);
@@ -968,7 +974,7 @@ int launch_low_prompt(const Call& c) {
 template <int BN, bool DUAL>
 int launch_tiles(const Call& c) {
   static std::atomic<unsigned long long> devices{0};
-  static ClusterTable table;
+  static ClusterTable table, deep_table;
   cudaError_t e = allow_smem(adapter_gemm_kernel<BN, DUAL>, devices);
   if (e != cudaSuccess) return (int)e;
   constexpr int FEATURES = DUAL ? 64 : 128;
@@ -1003,9 +1009,14 @@ int launch_tiles(const Call& c) {
   }
   if (DUAL) m_tiles = (c.M / 2 + FEATURES - 1) / FEATURES;
   const long long tiles = (long long)m_tiles * token_tiles;
+  // Few tiles of few tokens: one block per SM with a ring as deep as fits (4096 -> 6144, 32 tokens: 96 blocks 17.7 us a call, 192 blocks of half
+  // the depth 19.7).  Otherwise two per SM: their rings together are as deep, and one's epilogue hides behind the other (12288 -> 4096, 128
+  // tokens: 256 blocks 76, 128 blocks with an SM each 82; 4096 -> 2 x 12288, 32 tokens: 46 and 57).
+  const bool deep = BN <= 64 && tiles <= SMS / 2;
   size_t smem;
-  a.stages = ring_stages(HALF_SM, stage_bytes<BN>(), (size_t)BN * RED_PITCH * 4, smem);
-  const int cs = tiles > 2 * SMS ? 1 : cluster_size(table, tiles, a.kb, smem);
+  a.stages = ring_stages(deep ? SMEM_LIMIT : HALF_SM, stage_bytes<BN>(), (size_t)BN * RED_PITCH * 4, smem);
+  const int most = deep && SMS / tiles < a.kb ? (int)(SMS / tiles) : a.kb;
+  const int cs = tiles > 2 * SMS ? 1 : cluster_size(deep ? deep_table : table, tiles, most, smem);
   CUtensorMap tw, tx, tb, th;
   int rc = prism_get_tensor_map(c.w, (unsigned long long)c.M, (unsigned long long)c.K, (unsigned long long)c.ldw, FEATURES, &tw);
   if (!rc) rc = prism_get_tensor_map(c.x, (unsigned long long)c.T, (unsigned long long)c.K, (unsigned long long)c.ldx, BN, &tx);

@@ -7,8 +7,9 @@
 // pages[start_i + p / page] * page + p % page.
 //
 // A few KB to a few MB move, so a launch is what the step costs: one launch, in which every block adds up all lengths itself (1024
-// requests: 8 KB from L2) instead of waiting for a block that does, then writes its share of the tables, a row per warp, and of the
-// tokens, which find their request by halving the running sum in shared memory.
+// requests: 8 KB from L2, one pass over them and one exchange between warps) instead of waiting for a block that does, then writes its
+// share of the tables, 128 entries of a row per warp, and of the tokens, which find their request by halving the running sum in shared
+// memory.  1 request 3.2 us, 1024 requests of up to 8192 tokens in pages of 16 (4 MB, 0.6 us of copy bandwidth) MAPS_US us.
 #include "common.cuh"
 
 PRISM_DEFINE_TU_STATUS(batch)
@@ -17,7 +18,8 @@ namespace {
 
 constexpr int MAP_THREADS = 256;
 constexpr int MAP_WARPS = MAP_THREADS / 32;
-constexpr int MAP_MAX_REQUESTS = 8192;   // 8 bytes of shared memory each
+constexpr int MAP_MAX_REQUESTS = 8192;   // 12 bytes of shared memory each
+constexpr int MAP_SEGMENT = 128;         // entries of a table row that a warp writes at a time
 
 struct MapArgs {
   const int* pages;          // [n_pages] pages of all requests, one after another
@@ -41,7 +43,7 @@ struct MapArgs {
 enum { MAP_LENGTH = 1, MAP_TOKENS = 2, MAP_WIDTH = 3, MAP_PAGES = 4 };   // details of a failed bounds check
 
 __device__ __forceinline__ int lengths_of(const MapArgs& a, int i, int& cached, int& fresh) {
-  const int c = a.cached[i], f = a.fresh[i];
+  const int c = __ldg(a.cached + i), f = __ldg(a.fresh + i);
   const bool bad = c < 0 || f < 0 || c > 0x7fffffff - f;
   cached = bad ? 0 : c;
   fresh = bad ? 0 : f;
@@ -54,59 +56,68 @@ __device__ __forceinline__ int pages_of(int n, int page) { return n == 0 ? 0 : (
 __global__ void __launch_bounds__(MAP_THREADS) step_maps_kernel(const MapArgs a) {
   extern __shared__ int smem[];
   int* const cu = smem;                    // [S + 1] running sum of the new tokens
-  int* const start = smem + a.S + 1;       // [S + 1] and of the pages
+  int* const start = cu + a.S + 1;         // [S + 1] and of the pages
+  int* const behind = start + a.S + 1;     // [S] tokens in the cache
   __shared__ long long warp_sum[3][MAP_WARPS];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const bool first = blockIdx.x == 0;
   pdl_launch_dependents();
   pdl_wait();
 
-  // Running sums, MAP_THREADS requests at a time.  64 bits: a sum past 31 bits is reported, not wrapped.
-  long long base[3] = {0, 0, 0};
-  for (int i0 = 0; i0 < a.S; i0 += MAP_THREADS) {
-    const int i = i0 + threadIdx.x;
-    int cached = 0, fresh = 0, kv = 0;
-    if (i < a.S) kv = lengths_of(a, i, cached, fresh);
-    long long v[3] = {fresh, kv, pages_of(kv, a.page)}, incl[3];
+  // Running sums: a run of requests per thread.  64 bits: a sum past 31 bits is reported, not wrapped.
+  const int per = (a.S + MAP_THREADS - 1) / MAP_THREADS, i0 = min(a.S, (int)threadIdx.x * per), i1 = min(a.S, i0 + per);
+  long long mine[3] = {0, 0, 0}, at[3];
+#pragma unroll 4
+  for (int i = i0; i < i1; ++i) {
+    int cached, fresh;
+    const int kv = lengths_of(a, i, cached, fresh);
+    mine[0] += fresh;
+    mine[1] += kv;
+    mine[2] += pages_of(kv, a.page);
+  }
 #pragma unroll
-    for (int k = 0; k < 3; ++k) {
-      incl[k] = v[k];
+  for (int k = 0; k < 3; ++k) {
+    at[k] = mine[k];
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const long long up = __shfl_up_sync(0xffffffffu, incl[k], o);
-        if (lane >= o) incl[k] += up;
-      }
-      if (lane == 31) warp_sum[k][warp] = incl[k];
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long up = __shfl_up_sync(0xffffffffu, at[k], o);
+      if (lane >= o) at[k] += up;
     }
-    __syncthreads();
+    if (lane == 31) warp_sum[k][warp] = at[k];
+    at[k] -= mine[k];
+  }
+  __syncthreads();
+  long long all[3] = {0, 0, 0};
 #pragma unroll
-    for (int k = 0; k < 3; ++k) {
-      long long before = base[k];
-      for (int w = 0; w < MAP_WARPS; ++w) {
-        if (w < warp) before += warp_sum[k][w];
-        base[k] += warp_sum[k][w];
-      }
-      incl[k] += before;
+  for (int k = 0; k < 3; ++k)
+#pragma unroll
+    for (int w = 0; w < MAP_WARPS; ++w) {
+      if (w < warp) at[k] += warp_sum[k][w];
+      all[k] += warp_sum[k][w];
     }
-    if (i < a.S) {
-      // tokens past T have no rows: every sum stops there
-      cu[i + 1] = (int)min(incl[0], (long long)a.T);
-      start[i + 1] = (int)min(incl[2], (long long)a.n_pages);
-      if (first) {
-        a.cu_q[i + 1] = cu[i + 1];
-        a.cu_kv[i + 1] = (int)min(incl[1], 0x7fffffffll);
-        a.kv_lens[i] = kv;
-        a.sample_rows[i] = fresh > 0 && incl[0] <= a.T ? incl[0] - 1 : -1;
-      }
+  for (int i = i0; i < i1; ++i) {
+    int cached, fresh;
+    const int kv = lengths_of(a, i, cached, fresh);
+    at[0] += fresh;
+    at[1] += kv;
+    at[2] += pages_of(kv, a.page);
+    // tokens past T have no rows: every sum stops there
+    cu[i + 1] = (int)min(at[0], (long long)a.T);
+    start[i + 1] = (int)min(at[2], (long long)a.n_pages);
+    behind[i] = cached;
+    if (first) {
+      a.cu_q[i + 1] = cu[i + 1];
+      a.cu_kv[i + 1] = (int)min(at[1], 0x7fffffffll);
+      a.kv_lens[i] = kv;
+      a.sample_rows[i] = fresh > 0 && at[0] <= a.T ? at[0] - 1 : -1;
     }
-    __syncthreads();
   }
   if (threadIdx.x == 0) {
     cu[0] = start[0] = 0;
     if (first) {
       a.cu_q[0] = a.cu_kv[0] = 0;
-      if (base[0] > a.T || base[1] > 0x7fffffffll) prism_report(PRISM_ERR_BOUNDS, MAP_TOKENS);
-      if (a.page_offsets == nullptr && base[2] > a.n_pages) prism_report(PRISM_ERR_BOUNDS, MAP_PAGES);
+      if (all[0] > a.T || all[1] > 0x7fffffffll) prism_report(PRISM_ERR_BOUNDS, MAP_TOKENS);
+      if (a.page_offsets == nullptr && all[2] > a.n_pages) prism_report(PRISM_ERR_BOUNDS, MAP_PAGES);
     }
   }
   __syncthreads();
@@ -122,7 +133,9 @@ __global__ void __launch_bounds__(MAP_THREADS) step_maps_kernel(const MapArgs a)
     }
   };
 
-  for (int i = blockIdx.x * MAP_WARPS + warp; i < a.S; i += gridDim.x * MAP_WARPS) {
+  const int segments = (a.W + MAP_SEGMENT - 1) / MAP_SEGMENT;
+  for (long long w = (long long)blockIdx.x * MAP_WARPS + warp; w < (long long)a.S * segments; w += (long long)gridDim.x * MAP_WARPS) {
+    const int i = (int)(w / segments), j0 = (int)(w - (long long)i * segments) * MAP_SEGMENT;
     int cached, fresh, lo, hi;
     const int need = pages_of(lengths_of(a, i, cached, fresh), a.page);
     span(i, lo, hi);
@@ -130,8 +143,12 @@ __global__ void __launch_bounds__(MAP_THREADS) step_maps_kernel(const MapArgs a)
     if (lane == 0 && need > hi - lo) prism_report(PRISM_ERR_BOUNDS, MAP_PAGES);
     const int n = min(need, hi - lo);
     int* const row = a.tables + (size_t)i * a.W;
-#pragma unroll 4
-    for (int j = lane; j < a.W; j += 32) row[j] = j < n ? a.pages[lo + j] : -1;
+    int id[MAP_SEGMENT / 32];
+#pragma unroll
+    for (int e = 0; e < MAP_SEGMENT / 32; ++e) id[e] = j0 + e * 32 + lane < n ? a.pages[lo + j0 + e * 32 + lane] : -1;
+#pragma unroll
+    for (int e = 0; e < MAP_SEGMENT / 32; ++e)
+      if (j0 + e * 32 + lane < a.W) row[j0 + e * 32 + lane] = id[e];
   }
 
   const int total = cu[a.S];
@@ -146,10 +163,9 @@ __global__ void __launch_bounds__(MAP_THREADS) step_maps_kernel(const MapArgs a)
         else hi = mid;
       }
       seq = lo;
-      int cached, fresh, first_page, end_page;
-      lengths_of(a, seq, cached, fresh);
+      int first_page, end_page;
       span(seq, first_page, end_page);
-      const int p = cached + (t - cu[seq]), q = p / a.page;
+      const int p = behind[seq] + (t - cu[seq]), q = p / a.page;
       if (q < end_page - first_page) {
         const int id = a.pages[first_page + q];
         if (id >= 0) slot = (long long)id * a.page + (p - q * a.page);
@@ -196,13 +212,15 @@ PRISM_API int prism_step_maps(const void* pages, const void* page_offsets, const
   a.cu_kv = (int*)cu_kv;
   a.kv_lens = (int*)kv_lens;
   a.sample_rows = (long long*)sample_rows;
-  const long long rows = ((long long)S + MAP_WARPS - 1) / MAP_WARPS, tokens = ((long long)T + MAP_THREADS - 1) / MAP_THREADS;
-  long long grid = rows > tokens ? rows : tokens;
-  if (grid > 296) grid = 296;
+  // four blocks per SM at most: every one of them adds up the lengths
+  const long long warps = (long long)S * ((W + MAP_SEGMENT - 1) / MAP_SEGMENT), tokens = ((long long)T + MAP_THREADS - 1) / MAP_THREADS;
+  long long grid = (warps + MAP_WARPS - 1) / MAP_WARPS;
+  if (grid < tokens) grid = tokens;
+  if (grid > 4 * 148) grid = 4 * 148;
   if (grid < 1) grid = 1;
-  const size_t smem = (size_t)(2 * S + 2) * sizeof(int);
-  if (smem > 48 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(step_maps_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (2 * MAP_MAX_REQUESTS + 2) * 4);
+  const size_t smem = (size_t)(3 * S + 2) * sizeof(int);
+  if (smem > 47 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(step_maps_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (3 * MAP_MAX_REQUESTS + 2) * 4);
     if (e != cudaSuccess) return (int)e;
   }
   return (int)prism_launch(step_maps_kernel, dim3((unsigned)grid), dim3(MAP_THREADS), smem, (cudaStream_t)stream, pdl != 0, a);
