@@ -117,14 +117,16 @@ struct LowArgs {
   int T, kb, capacity, all_panels, tile_rows, stages;
 };
 
-// The place of every token of a tile in the list of adapters, and that adapter's scale.
+// The place of every token of a tile in the list of adapters, and the list itself (-1 behind its end).
 template <int TOKENS>
-__device__ __forceinline__ void load_owners(const LowArgs& a, int* who, float* scale, int token0, const int* list) {
-  for (int c = threadIdx.x; c < TOKENS; c += TC_THREADS) {
-    const int j = token0 + c < a.T ? a.index[token0 + c] : -1;
-    who[c] = j;
-    scale[c] = j >= 0 ? a.scale[list[j]] : 0.0f;
-  }
+__device__ __forceinline__ void load_owners(const LowArgs& a, int* who, int* slot, int token0, int tile) {
+  for (int c = threadIdx.x; c < TOKENS; c += TC_THREADS) who[c] = token0 + c < a.T ? a.index[token0 + c] : -1;
+  for (int j = threadIdx.x; j < a.capacity; j += TC_THREADS) slot[j] = a.lists[(size_t)tile * a.capacity + j];
+}
+// And the scale of every token's adapter; by the epilogue warps, while the sums are under way.
+template <int TOKENS>
+__device__ __forceinline__ void load_scales(const LowArgs& a, const int* who, const int* slot, float* scale) {
+  for (int c = threadIdx.x - 64; c < TOKENS; c += TC_THREADS - 64) scale[c] = who[c] >= 0 ? a.scale[slot[who[c]]] : 0.0f;
 }
 
 // Sum over the cluster of four floats that every CTA keeps at the same place.
@@ -189,8 +191,7 @@ adapter_low_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 1);
   const int warp = uniform_warp(), lane = threadIdx.x & 31;
   const int panels = min(a.counts[0], a.capacity) * a.all_panels;
-  const int* const list = a.lists;
-  __shared__ int who[BN];
+  __shared__ int who[BN], slot[BN];   // no more adapters than tokens
   __shared__ float scale[BN];
 
   const int kb0 = part_begin(a.kb, blockIdx.z, gridDim.z), kb1 = part_begin(a.kb, blockIdx.z + 1, gridDim.z);
@@ -210,7 +211,7 @@ adapter_low_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
     tmem_alloc(tmem_slot, TMEM_COLS);
     tmem_relinquish();
   }
-  load_owners<BN>(a, who, scale, 0, list);
+  load_owners<BN>(a, who, slot, 0, 0);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -227,7 +228,7 @@ adapter_low_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
 #pragma unroll
         for (int i = 0; i < G * 8; ++i) {
           const int p = p0 + min(i, np - 1), j = p / a.all_panels;
-          row[i] = (list[j] * a.all_panels + (p - j * a.all_panels)) * 16;
+          row[i] = (slot[j] * a.all_panels + (p - j * a.all_panels)) * 16;
         }
         for (int kb = kb0; kb < kb1; ++kb) {
           ok = mbar_wait(&empty[s], parity ^ 1, 1);
@@ -270,6 +271,7 @@ adapter_low_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
         if (ok) tc_commit(acc_full);
       }
     } else {
+      if (round == 0) load_scales<BN>(a, who, slot, scale);
       // rows of unused panels hold what earlier loads left; nothing reads them
       ok = ok && __all_sync(0xffffffffu, mbar_wait(acc_full, round & 1, 3));
       if (ok) {
@@ -313,14 +315,14 @@ adapter_low_prompt_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_
   const int warp = uniform_warp(), lane = threadIdx.x & 31;
   const int token0 = blockIdx.y * 128, tile = token0 / PLAN_TILE;
   const int count = min(a.counts[tile], a.capacity);
-  const int* const list = a.lists + (size_t)tile * a.capacity;
-  __shared__ int who[128];
+  __shared__ int who[128], slot[PLAN_TILE];
   __shared__ float scale[128];
   __shared__ short place[PLAN_TILE], active[128];   // of the list's adapters: which of the active ones, -1: none; and back
   __shared__ int n_active;
   for (int j = threadIdx.x; j < count; j += TC_THREADS) place[j] = -1;
 
   const int kb0 = part_begin(a.kb, blockIdx.z, gridDim.z), kb1 = part_begin(a.kb, blockIdx.z + 1, gridDim.z);
+  const int pre = count > 0 ? min(stages, kb1 - kb0) : 0;   // as above
   if (warp == 0 && elect_one()) {
     for (int s = 0; s < stages; ++s) {
       mbar_init(&full[s], 1);
@@ -328,14 +330,14 @@ adapter_low_prompt_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_
     }
     mbar_init(acc_full, 1);
     fence_barrier_init();
+    for (int i = 0; i < pre; ++i) tma_load_2d(smem + (size_t)i * STAGE, &tmX, &full[i], (kb0 + i) * 64, token0);
     tma_prefetch_desc(&tmA);
-    tma_prefetch_desc(&tmX);
   }
   if (warp == 1) {
     tmem_alloc(tmem_slot, TMEM_COLS);
     tmem_relinquish();
   }
-  load_owners<128>(a, who, scale, token0, list);
+  load_owners<128>(a, who, slot, token0, tile);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -359,6 +361,12 @@ adapter_low_prompt_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_
   }
   __syncthreads();
   const int panels = n_active * a.all_panels;
+  if (panels == 0 && warp == 0 && elect_one()) {   // the tokens loaded ahead are not needed: only let them land
+    for (int i = 0; i < pre; ++i) {
+      mbar_expect_tx(&full[i], W_BYTES);
+      (void)mbar_wait(&full[i], 0, 4);
+    }
+  }
   if (warp >= 2) {   // zeros for adapters that only the tile's other 128 tokens have
     const int cs = gridDim.z, share = 128 / cs;
     bf16* const h = a.h + (size_t)tile * a.capacity * a.all_panels * a.tile_rows * 16;
@@ -380,14 +388,14 @@ adapter_low_prompt_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_
 #pragma unroll
         for (int i = 0; i < PASS; ++i) {
           const int p = p0 + min(i, np - 1), j = p / a.all_panels;
-          row[i] = (list[active[j]] * a.all_panels + (p - j * a.all_panels)) * 16;
+          row[i] = (slot[active[j]] * a.all_panels + (p - j * a.all_panels)) * 16;
         }
         for (int kb = kb0; kb < kb1; ++kb) {
           ok = mbar_wait(&empty[s], parity ^ 1, 1);
           if (!ok) break;
           uint8_t* const st = smem + (size_t)s * STAGE;
           mbar_expect_tx(&full[s], W_BYTES + np * 2048);
-          tma_load_2d(st, &tmX, &full[s], kb * 64, token0);
+          if (round > 0 || kb - kb0 >= pre) tma_load_2d(st, &tmX, &full[s], kb * 64, token0);
 #pragma unroll
           for (int i = 0; i < PASS; ++i)
             if (i < np) tma_load_2d(st + W_BYTES + i * 2048, &tmA, &full[s], kb * 64, row[i]);
@@ -417,6 +425,7 @@ adapter_low_prompt_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_
         if (ok) tc_commit(acc_full);
       }
     } else {
+      if (round == 0) load_scales<128>(a, who, slot, scale);
       const int q = warp & 3, c = q * 32 + lane, first_own = who[c] < 0 ? panels : place[who[c]] * a.all_panels;
       ok = ok && __all_sync(0xffffffffu, mbar_wait(acc_full, round & 1, 3));
       if (ok) {
@@ -845,7 +854,7 @@ __global__ void __launch_bounds__(F32_THREADS, 4) adapter_gemm_f32_kernel(const 
 }
 
 constexpr int SMS = 148;
-constexpr int SMEM_LIMIT = 232448 - 2048;   // 227 KB, 2 KB of it for static arrays
+constexpr int SMEM_LIMIT = 232448 - 4096;   // 227 KB, 4 KB of it for static arrays
 
 // Dynamic shared memory above 48 KB has to be allowed once per kernel and device.
 template <typename Kernel>
@@ -883,11 +892,12 @@ struct Call {
   long long ldo;
   void* h;
   int T, M, K, act, tile_rows;
+  int pair_tiles;        // tiles of the projection on pairs of SMs (0: another kernel runs it)
   cudaStream_t stream;
   bool pdl;
 };
 
-constexpr int HALF_SM = 112 * 1024 + 512;   // two such blocks share an SM: the projection streams weights beside the low-rank rows
+constexpr int HALF_SM = 111 * 1024;   // two such blocks share an SM: the projection streams weights beside the low-rank rows
 
 // The largest cluster of 8, 4 or 2 blocks along z, at most `most`, of which n fit the device at once; 1 if none does.  More clusters than fit
 // take a second round: 16 clusters of 8 blocks with an SM each took 22 us, 13 of them 11.6.  The count is asked for with an empty kernel: for
@@ -961,9 +971,12 @@ int launch_low_prompt(const Call& c) {
   const int tiles = (c.T + 127) / 128;
   size_t smem;
   a.stages = ring_stages(SMEM_LIMIT, W_BYTES + 16 * 2048, (size_t)16 * 128 * 20 * 4, smem);
-  // Half the SMs at most: the projection's pairs of SMs that walk one tile more than the others are its first blocks and start on the other
-  // half at once, the rest have as much time for the low-rank rows as a tile takes.
-  const int cs = 2 * tiles > SMS ? 1 : cluster_size(table, tiles, a.kb < SMS / 2 / tiles ? a.kb : SMS / 2 / tiles, smem);
+  // The projection's pairs of SMs that walk one tile more than the others are its first blocks.  Where there are SMs for them beside these
+  // blocks they start at once, and the others have as much time for the low-rank rows as a tile takes (8192 tokens, 4096 -> 6144 qkv: 64
+  // blocks, 300 us; 128 blocks, whose rows take half the time, 306).  Where most pairs walk one tile more the rows come first, as fast as may be.
+  const int more = c.pair_tiles % (SMS / 2), beside = SMS - 2 * (more ? more : SMS / 2);
+  const int room = tiles <= beside ? beside : SMS;
+  const int cs = tiles > room ? 1 : cluster_size(table, tiles, a.kb < room / tiles ? a.kb : room / tiles, smem);
   CUtensorMap ta, tx;
   int rc = prism_get_tensor_map(c.a, (unsigned long long)c.terms.slots * a.all_panels * 16, (unsigned long long)c.K, (unsigned long long)c.K, 16, &ta);
   if (!rc) rc = prism_get_tensor_map(c.x, (unsigned long long)c.T, (unsigned long long)c.K, (unsigned long long)c.ldx, 128, &tx);
@@ -1036,10 +1049,13 @@ int launch_decode(const Call& c) {
   return c.act ? launch_tiles<BN, true>(c) : launch_tiles<BN, false>(c);
 }
 
-int launch_prompt(const Call& c) {
+int launch_prompt(Call& c) {
+  const bool pair = prism_adapter_pair_fits(c.M, c.act != 0, c.terms, c.out, c.ldo, c.bias);
+  int bn;
+  c.pair_tiles = pair ? prism_adapter_pair_tiles(c.M, c.T, c.act != 0, c.terms, &bn) : 0;
   const int rc = launch_low_prompt(c);
   if (rc) return rc;
-  if (prism_adapter_pair_fits(c.M, c.act != 0, c.terms, c.out, c.ldo, c.bias))
+  if (pair)
     return prism_adapter_pair(c.w, c.x, c.out, c.M, c.T, c.K, c.ldw, c.ldx, c.ldo, c.bias, c.act != 0, c.act, c.terms, c.stream, true);
   return c.act ? launch_tiles<128, true>(c) : launch_tiles<128, false>(c);
 }

@@ -430,6 +430,7 @@ struct PrismAdapterTerms {
   PrismAdapterSections sec;
 };
 bool prism_adapter_pair_fits(int M, int dual, const PrismAdapterTerms& t, const void* out, long long ldo, const void* bias);
+int prism_adapter_pair_tiles(int M, int T, int dual, const PrismAdapterTerms& t, int* columns);   // and a tile's columns
 int prism_adapter_pair(const void* W, const void* X, void* out, int M, int T, int K, long long ldw, long long ldx, long long ldo,
                        const void* bias, int dual, int act, const PrismAdapterTerms& t, cudaStream_t stream, bool pdl);
 struct PrismLaunch {

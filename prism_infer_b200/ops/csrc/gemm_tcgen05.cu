@@ -938,6 +938,16 @@ bool prism_adapter_pair_fits(int M, int dual, const PrismAdapterTerms& t, const 
   return true;
 }
 
+// Tiles do not cross sections; those of a gated unit hold gates and their ups.
+int prism_adapter_pair_tiles(int M, int T, int dual, const PrismAdapterTerms& t, int* columns) {
+  const int m_tiles = (T + 255) / 256;
+  int widths[8], n = 0;
+  for (int s = 0; s < t.sec.n; ++s) widths[s] = t.sec.end[s] - (s ? t.sec.end[s - 1] : 0);
+  *columns = pair_columns(m_tiles, dual ? 1 : t.sec.n, dual ? &M : widths, dual != 0);
+  for (int s = 0; s < (dual ? 1 : t.sec.n); ++s) n += ((dual ? M : widths[s]) + *columns - 1) / *columns;
+  return m_tiles * n;
+}
+
 // W [M, K], X [T, K] bf16; out bf16 [T, ldo].  dual: W is gate rows and up rows, M / 2 each, out is act(gate) * up.
 int prism_adapter_pair(const void* W, const void* X, void* out, int M, int T, int K, long long ldw, long long ldx, long long ldo,
                        const void* bias, int dual, int act, const PrismAdapterTerms& t, cudaStream_t stream, bool pdl) {
@@ -964,17 +974,14 @@ int prism_adapter_pair(const void* W, const void* X, void* out, int M, int T, in
   d.b_groups = t.b_rows / 8;
   d.no_group = t.slots * t.panels * d.b_groups;
   d.sections = t.sec.n;
-  int widths[8];
-  for (int s = 0; s < t.sec.n; ++s) widths[s] = t.sec.end[s] - (s ? t.sec.end[s - 1] : 0);
-  a.bn = pair_columns(a.m_tiles, dual ? 1 : t.sec.n, dual ? &M : widths, dual != 0);
-  a.n_tiles = 0;
-  for (int s = 0; s < t.sec.n; ++s) {
+  const int tiles = prism_adapter_pair_tiles(M, T, dual, t, &a.bn);
+  a.n_tiles = tiles / a.m_tiles;
+  for (int s = 0, first = 0; s < t.sec.n; ++s) {
     d.start[s] = s == 0 ? 0 : t.sec.end[s - 1];
     d.end[s] = t.sec.end[s];
-    d.first_tile[s] = a.n_tiles;
-    a.n_tiles += (d.end[s] - d.start[s] + a.bn - 1) / a.bn;
+    d.first_tile[s] = first;
+    first += (d.end[s] - d.start[s] + a.bn - 1) / a.bn;
   }
-  if (dual) a.n_tiles = (M + a.bn - 1) / a.bn;
   const int stage_bytes = W_TILE_BYTES + a.bn * 64;
   a.stages = (SMEM_LIMIT - 1024 - 512 - PAIR_TURN_BYTES) / stage_bytes;
   if (a.stages > 12) a.stages = 12;
@@ -987,7 +994,7 @@ int prism_adapter_pair(const void* W, const void* X, void* out, int M, int T, in
   if (rc) return rc;
   const cudaError_t e = cudaFuncSetAttribute(gemm_pair_adapter_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_LIMIT);
   if (e != cudaSuccess) return (int)e;
-  const int tiles = a.m_tiles * a.n_tiles, pairs = sm_count() / 2;
+  const int pairs = sm_count() / 2;
   return (int)prism_launch(gemm_pair_adapter_kernel, dim3(2 * (tiles < pairs ? tiles : pairs)), dim3(PAIR_THREADS), smem, stream, pdl, tx, tw, th, tb,
                            a, d);
 }
