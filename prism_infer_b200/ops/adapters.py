@@ -11,6 +11,7 @@ CUDA tensors run ``csrc/adapters.cu`` beside the GEMM kernels; CPU tensors the p
 from __future__ import annotations
 
 import ctypes
+import math
 from dataclasses import dataclass
 from typing import Optional, Sequence, Union
 
@@ -18,7 +19,7 @@ import torch
 import torch.nn.functional as F
 
 from . import GLU_ACTS, _p, _pdl, _s, glu_act, native
-from .batch import check_device
+from .batch import MAX_ROWS, check_device
 
 PANEL = 16             # ranks are padded to multiples of this
 TILE_TOKENS = 256      # tokens that share a list of adapters
@@ -58,6 +59,7 @@ class AdapterPool:
         ends = [sum(sections[:i + 1]) for i in range(len(sections))]
         self._ends = (ctypes.c_int * len(ends))(*ends)
 
+    @torch.no_grad()
     def load(self, slot: int, a, b, scale: float = 1.0) -> None:
         """``a``: ``[r, in_features]`` and ``b``: ``[features, r]``, or one of each per section; ranks up to the pool's.  The copies are
         made on the current stream.  Factors that are not finite are refused: tokens of other adapters meet them as products with
@@ -72,20 +74,18 @@ class AdapterPool:
                 raise ValueError(f"factors {tuple(fa.shape)} and {tuple(fb.shape)} for {self.in_features} -> {m}")
             if not 1 <= fa.shape[0] <= self.rank:
                 raise ValueError(f"rank {fa.shape[0]}, the pool holds up to {self.rank}")
-        scale = float(scale)
-        if not torch.isfinite(torch.tensor(scale, dtype=torch.float32)) or not all(bool(torch.isfinite(f.to(self.dtype)).all()) for f in (*a, *b)):
-            raise ValueError("factors and scale must be finite")
-        self.clear(slot)
+        pa = torch.zeros(len(a), self.panels * PANEL, self.in_features, dtype=self.dtype, device=self.device)
+        pb = torch.zeros(self.rows, self.panels * PANEL, dtype=self.dtype, device=self.device)
         first = 0
         for i, (fa, fb, m) in enumerate(zip(a, b, self.sections)):
-            r, row = fa.shape[0], i * self.panels * PANEL
-            self.a[slot, row:row + r] = fa
-            rows = -(-m // 8) * 8
-            padded = torch.zeros(rows, self.panels * PANEL, dtype=self.dtype, device=self.device)
-            padded[:m, :r] = fb
-            self.b[slot, :, first:first + rows] = self._panels(padded.view(rows, self.panels, PANEL).transpose(0, 1))
-            first += rows
-        self.scale[slot] = scale
+            pa[i, :fa.shape[0]] = fa
+            pb[first:first + m, :fb.shape[1]] = fb
+            first += -(-m // 8) * 8
+        if not math.isfinite(ctypes.c_float(float(scale)).value) or not bool(torch.isfinite(pa).all() & torch.isfinite(pb).all()):
+            raise ValueError("factors and scale must be finite")
+        self.a[slot] = pa.view(self.low, self.in_features)
+        self.b[slot] = self._panels(pb.view(self.rows, self.panels, PANEL).transpose(0, 1))
+        self.scale[slot] = float(scale)
 
     def _panels(self, b: torch.Tensor) -> torch.Tensor:
         """``[panels, rows, 16]`` in the pool's order."""
@@ -99,6 +99,7 @@ class AdapterPool:
             b = b.reshape(b.shape[0], -1, 2, 8, 8).transpose(2, 3).reshape(b.shape)
         return b.transpose(0, 1).reshape(b.shape[1], -1)[:m]
 
+    @torch.no_grad()
     def clear(self, slot: int) -> None:
         """The slot adds nothing from here on."""
         if not 0 <= slot < self.slots:
@@ -121,14 +122,14 @@ class AdapterPlan:
 
 
 def plan(adapter: torch.Tensor, slots: int) -> AdapterPlan:
-    """Once per step, for every projection whose pool has ``slots`` slots.  ``adapter``: contiguous int32, one per token.  Slots out of
+    """Once per step, for every projection whose pool has ``slots`` slots; again when ``adapter`` has changed.  ``adapter``: contiguous int32, one per token.  Slots out of
     range count as none and set the ``adapters`` status word (``native.check_status``); on CPU they raise."""
     if adapter.dtype != torch.int32 or adapter.dim() != 1 or not adapter.is_contiguous():
         raise ValueError("adapter must be a contiguous one-dimensional int32 tensor")
     if not 1 <= slots <= MAX_SLOTS:
         raise ValueError(f"{slots} slots, one to {MAX_SLOTS}")
     T = adapter.shape[0]
-    if T >= 2 ** 31 - TILE_TOKENS:
+    if T > MAX_ROWS:
         raise ValueError(f"{T} tokens")
     tiles, capacity = -(-T // TILE_TOKENS), min(slots, TILE_TOKENS, T)
     if not adapter.is_cuda:

@@ -17,6 +17,7 @@ import torch
 from . import _p, _pdl, _s, native
 
 MAX_REQUESTS = 8192
+MAX_ROWS = 1 << 30
 
 
 @dataclass
@@ -73,8 +74,8 @@ def step_maps(pages: torch.Tensor, cached: torch.Tensor, fresh: torch.Tensor, *,
         raise ValueError(f"page {page} and width {width} must be positive, tokens {tokens} not negative")
     if S > MAX_REQUESTS:
         raise ValueError(f"{S} requests, at most {MAX_REQUESTS} in a step")
-    if tokens >= 2 ** 31 or width >= 2 ** 31 or page >= 2 ** 31 or pages.shape[0] >= 2 ** 31:
-        raise ValueError("sizes must fit 32 bits")
+    if tokens > MAX_ROWS or width > MAX_ROWS or page >= 2 ** 31 or pages.shape[0] >= 2 ** 31:
+        raise ValueError(f"at most {MAX_ROWS} tokens and table entries, pages and their list within 31 bits")
     if not cached.is_cuda:
         return _step_maps_cpu(pages, cached, fresh, page, tokens, width, page_offsets, shift, adapter)
     check_device(cached)

@@ -115,13 +115,14 @@ struct LowArgs {
   const float* scale;    // [slots]
   bf16* h;               // [tiles][capacity][all_panels] panels of tile_rows tokens
   int T, kb, capacity, all_panels, tile_rows, stages;
+  int run;               // panels that one copy moves: a divisor of all_panels, since an adapter's rows of A lie together
 };
 
-// The place of every token of a tile in the list of adapters, and the list itself (-1 behind its end).
-template <int TOKENS>
+// The place of every token of a tile in the list of adapters, and the list itself (-1 behind its end), of which no more than MOST are in use.
+template <int TOKENS, int MOST>
 __device__ __forceinline__ void load_owners(const LowArgs& a, int* who, int* slot, int token0, int tile) {
   for (int c = threadIdx.x; c < TOKENS; c += TC_THREADS) who[c] = token0 + c < a.T ? a.index[token0 + c] : -1;
-  for (int j = threadIdx.x; j < a.capacity; j += TC_THREADS) slot[j] = a.lists[(size_t)tile * a.capacity + j];
+  for (int j = threadIdx.x; j < min(a.capacity, MOST); j += TC_THREADS) slot[j] = a.lists[(size_t)tile * a.capacity + j];
 }
 // And the scale of every token's adapter; by the epilogue warps, while the sums are under way.
 template <int TOKENS>
@@ -190,13 +191,14 @@ adapter_low_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
   uint64_t* acc_full = empty + stages;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 1);
   const int warp = uniform_warp(), lane = threadIdx.x & 31;
-  const int panels = min(a.counts[0], a.capacity) * a.all_panels;
+  const int panels = min(a.counts[0], min(a.capacity, BN)) * a.all_panels;
   __shared__ int who[BN], slot[BN];   // no more adapters than tokens
   __shared__ float scale[BN];
 
   const int kb0 = part_begin(a.kb, blockIdx.z, gridDim.z), kb1 = part_begin(a.kb, blockIdx.z + 1, gridDim.z);
   // the first tokens are under way before the list of adapters is read; their bytes are announced with those of the factors
-  const int pre = (int)blockIdx.x * G * 8 < panels ? min(stages, kb1 - kb0) : 0;
+  const int pass = G * 8 / a.run * a.run;   // panels of a pass
+  const int pre = (int)blockIdx.x * pass < panels ? min(stages, kb1 - kb0) : 0;
   if (warp == 0 && elect_one()) {
     for (int s = 0; s < stages; ++s) {
       mbar_init(&full[s], 1);
@@ -211,7 +213,7 @@ adapter_low_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
     tmem_alloc(tmem_slot, TMEM_COLS);
     tmem_relinquish();
   }
-  load_owners<BN>(a, who, slot, 0, 0);
+  load_owners<BN, BN>(a, who, slot, 0, 0);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -220,14 +222,14 @@ adapter_low_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
   int s = 0, round = 0;   // ring stage; passes done
   uint32_t parity = 0;    // of the full barriers (MMA); the producer waits for the phase before
   bool ok = true;         // this thread's role goes on; after a wait that ran out it only keeps step with the cluster
-  for (int p0 = blockIdx.x * G * 8; p0 < panels; p0 += gridDim.x * G * 8, ++round) {
-    const int np = min(G * 8, panels - p0);
+  for (int p0 = blockIdx.x * pass; p0 < panels; p0 += gridDim.x * pass, ++round) {
+    const int np = min(pass, panels - p0);
     if (warp == 0) {
       if (elect_one() && ok) {
         int row[G * 8];
 #pragma unroll
         for (int i = 0; i < G * 8; ++i) {
-          const int p = p0 + min(i, np - 1), j = p / a.all_panels;
+          const int p = p0 + min(i * a.run, np - 1), j = p / a.all_panels;
           row[i] = (slot[j] * a.all_panels + (p - j * a.all_panels)) * 16;
         }
         for (int kb = kb0; kb < kb1; ++kb) {
@@ -238,7 +240,7 @@ adapter_low_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
           if (round > 0 || kb - kb0 >= pre) tma_load_2d(st + X_AT, &tmX, &full[s], kb * 64, 0);
 #pragma unroll
           for (int i = 0; i < G * 8; ++i)
-            if (i < np) tma_load_2d(st + i * 2048, &tmA, &full[s], kb * 64, row[i]);
+            if (i * a.run < np) tma_load_2d(st + i * a.run * 2048, &tmA, &full[s], kb * 64, row[i]);
           if (++s == stages) s = 0, parity ^= 1;
         }
         if (!ok) {
@@ -296,21 +298,24 @@ adapter_low_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
   }
 }
 
+constexpr int LOW_PASS = 16, LOW_STAGES = 12;
+constexpr int LOW_PITCH = 20;            // floats of a row of 16 sums, without bank conflicts
+constexpr int LOW_RING = 208 * 1024;     // bytes; the sums of a pass (160 KB) take the same place
+
 // Prompts, 128 tokens: the tokens are the MMA's rows and up to 16 panels its columns, those of the adapters that these tokens have, so that a
 // k-block moves the tokens once and the factors of these adapters; the panels of the tile's other adapters get zeros.  Cluster (1, 1, CS)
 // splits K.
 __global__ void __launch_bounds__(TC_THREADS, 1)
 adapter_low_prompt_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmX, const LowArgs a) {
-  constexpr int PASS = 16, STAGE = W_BYTES + PASS * 2048, TMEM_COLS = PASS * 16, PITCH = 20;   // 20: rows of 16 floats without bank conflicts
+  constexpr int PASS = LOW_PASS, TMEM_COLS = PASS * 16, PITCH = LOW_PITCH;
   pdl_wait();
   pdl_launch_dependents();   // as above
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   float* const red = reinterpret_cast<float*>(smem);   // [panel of the pass][token][PITCH], in the ring's memory
-  const int stages = a.stages;
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + (size_t)stages * STAGE);
-  uint64_t* empty = full + stages;
-  uint64_t* acc_full = empty + stages;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + LOW_RING);
+  uint64_t* empty = full + LOW_STAGES;
+  uint64_t* acc_full = empty + LOW_STAGES;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 1);
   const int warp = uniform_warp(), lane = threadIdx.x & 31;
   const int token0 = blockIdx.y * 128, tile = token0 / PLAN_TILE;
@@ -322,6 +327,8 @@ adapter_low_prompt_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_
   for (int j = threadIdx.x; j < count; j += TC_THREADS) place[j] = -1;
 
   const int kb0 = part_begin(a.kb, blockIdx.z, gridDim.z), kb1 = part_begin(a.kb, blockIdx.z + 1, gridDim.z);
+  // as many stages as the ring holds for the panels that these tokens may have
+  const int pass = PASS / a.run * a.run, stage = W_BYTES + min(pass, count * a.all_panels) * 2048, stages = min(LOW_STAGES, LOW_RING / stage);
   const int pre = count > 0 ? min(stages, kb1 - kb0) : 0;   // as above
   if (warp == 0 && elect_one()) {
     for (int s = 0; s < stages; ++s) {
@@ -330,14 +337,14 @@ adapter_low_prompt_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_
     }
     mbar_init(acc_full, 1);
     fence_barrier_init();
-    for (int i = 0; i < pre; ++i) tma_load_2d(smem + (size_t)i * STAGE, &tmX, &full[i], (kb0 + i) * 64, token0);
+    for (int i = 0; i < pre; ++i) tma_load_2d(smem + (size_t)i * stage, &tmX, &full[i], (kb0 + i) * 64, token0);
     tma_prefetch_desc(&tmA);
   }
   if (warp == 1) {
     tmem_alloc(tmem_slot, TMEM_COLS);
     tmem_relinquish();
   }
-  load_owners<128>(a, who, slot, token0, tile);
+  load_owners<128, PLAN_TILE>(a, who, slot, token0, tile);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -380,25 +387,25 @@ adapter_low_prompt_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_
   int s = 0, round = 0;
   uint32_t parity = 0;
   bool ok = true;
-  for (int p0 = 0; p0 < panels; p0 += PASS, ++round) {
-    const int np = min(PASS, panels - p0);
+  for (int p0 = 0; p0 < panels; p0 += pass, ++round) {
+    const int np = min(pass, panels - p0);
     if (warp == 0) {
       if (elect_one() && ok) {
         int row[PASS];
 #pragma unroll
         for (int i = 0; i < PASS; ++i) {
-          const int p = p0 + min(i, np - 1), j = p / a.all_panels;
+          const int p = p0 + min(i * a.run, np - 1), j = p / a.all_panels;
           row[i] = (slot[active[j]] * a.all_panels + (p - j * a.all_panels)) * 16;
         }
         for (int kb = kb0; kb < kb1; ++kb) {
           ok = mbar_wait(&empty[s], parity ^ 1, 1);
           if (!ok) break;
-          uint8_t* const st = smem + (size_t)s * STAGE;
+          uint8_t* const st = smem + (size_t)s * stage;
           mbar_expect_tx(&full[s], W_BYTES + np * 2048);
           if (round > 0 || kb - kb0 >= pre) tma_load_2d(st, &tmX, &full[s], kb * 64, token0);
 #pragma unroll
           for (int i = 0; i < PASS; ++i)
-            if (i < np) tma_load_2d(st + W_BYTES + i * 2048, &tmA, &full[s], kb * 64, row[i]);
+            if (i * a.run < np) tma_load_2d(st + W_BYTES + i * a.run * 2048, &tmA, &full[s], kb * 64, row[i]);
           if (++s == stages) s = 0, parity ^= 1;
         }
         if (!ok) {
@@ -415,7 +422,7 @@ adapter_low_prompt_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_
           ok = mbar_wait(&full[s], parity, 2);
           if (!ok) break;
           tc_fence_after();
-          const uint32_t st = smem_u32(smem + (size_t)s * STAGE);
+          const uint32_t st = smem_u32(smem + (size_t)s * stage);
           const uint64_t da = umma_desc_sw128(st), db = umma_desc_sw128(st + W_BYTES);
 #pragma unroll
           for (int k = 0; k < 4; ++k) tc_mma_f16(tmem, da + 2 * k, db + 2 * k, idesc, kb != kb0 || k != 0);
@@ -938,9 +945,17 @@ int cluster_size(ClusterTable& table, long long n, int most, size_t smem) {
   return 1;
 }
 
-LowArgs low_args(const Call& c) {
+// The longest run of panels that leaves at most `unused` of a pass empty.  A copy per panel kept a prompt's issuing thread busy for longer than
+// the copies took (13 of them a k-block, 8192 tokens: 48 us; in runs of 6 panels 38).
+int panel_run(int all_panels, int pass, int unused) {
+  for (int run = all_panels < pass ? all_panels : pass; run > 1; --run)
+    if (all_panels % run == 0 && pass % run <= unused) return run;
+  return 1;
+}
+
+LowArgs low_args(const Call& c, int pass, int unused) {
   return LowArgs{c.terms.lists, c.terms.counts, c.index, c.scale, (bf16*)c.h, c.T, (c.K + 63) / 64, c.terms.capacity, c.terms.panels * c.terms.sec.n,
-                 c.tile_rows, 0};
+                 c.tile_rows, 0, panel_run(c.terms.panels * c.terms.sec.n, pass, unused)};
 }
 
 template <int BN, int G>
@@ -949,14 +964,14 @@ int launch_low(const Call& c) {
   static ClusterTable table;
   cudaError_t e = allow_smem(adapter_low_kernel<BN, G>, devices);
   if (e != cudaSuccess) return (int)e;
-  LowArgs a = low_args(c);
-  const int most = (a.capacity * a.all_panels + G * 8 - 1) / (G * 8);   // a step may bring as many adapters as tokens
+  LowArgs a = low_args(c, G * 8, 0);
+  const int pass = G * 8 / a.run * a.run, most = (a.capacity * a.all_panels + pass - 1) / pass;   // a step may bring as many adapters as tokens
   size_t smem;
   a.stages = ring_stages(G == 1 ? HALF_SM : SMEM_LIMIT, G * W_BYTES + BN * 128, (size_t)BN * (G * 128 + 4) * 4, smem);
   const int cs = most > SMS ? 1 : cluster_size(table, most, a.kb < SMS / most ? a.kb : SMS / most, smem);
   const int gx = SMS / cs < most ? SMS / cs : most;
   CUtensorMap ta, tx;
-  int rc = prism_get_tensor_map(c.a, (unsigned long long)c.terms.slots * a.all_panels * 16, (unsigned long long)c.K, (unsigned long long)c.K, 16, &ta);
+  int rc = prism_get_tensor_map(c.a, (unsigned long long)c.terms.slots * a.all_panels * 16, (unsigned long long)c.K, (unsigned long long)c.K, 16 * a.run, &ta);
   if (!rc) rc = prism_get_tensor_map(c.x, (unsigned long long)c.T, (unsigned long long)c.K, (unsigned long long)c.ldx, BN, &tx);
   if (rc) return rc;
   return (int)prism_launch_clusters(adapter_low_kernel<BN, G>, dim3(gx, 1, cs), dim3(TC_THREADS), smem, c.stream, c.pdl, cs, ta, tx, a);
@@ -967,10 +982,10 @@ int launch_low_prompt(const Call& c) {
   static ClusterTable table;
   cudaError_t e = allow_smem(adapter_low_prompt_kernel, devices);
   if (e != cudaSuccess) return (int)e;
-  LowArgs a = low_args(c);
+  LowArgs a = low_args(c, LOW_PASS, LOW_PASS / 4);
   const int tiles = (c.T + 127) / 128;
-  size_t smem;
-  a.stages = ring_stages(SMEM_LIMIT, W_BYTES + 16 * 2048, (size_t)16 * 128 * 20 * 4, smem);
+  static_assert(LOW_PASS * 128 * LOW_PITCH * 4 <= LOW_RING, "the sums fit the ring");
+  const size_t smem = 1024 + LOW_RING + (2 * LOW_STAGES + 1) * 8 + 16;
   // The projection's pairs of SMs that walk one tile more than the others are its first blocks.  Where there are SMs for them beside these
   // blocks they start at once, and the others have as much time for the low-rank rows as a tile takes (8192 tokens, 4096 -> 6144 qkv: 64
   // blocks, 300 us; 128 blocks, whose rows take half the time, 306).  Where most pairs walk one tile more the rows come first, as fast as may be.
@@ -978,7 +993,7 @@ int launch_low_prompt(const Call& c) {
   const int room = tiles <= beside ? beside : SMS;
   const int cs = tiles > room ? 1 : cluster_size(table, tiles, a.kb < room / tiles ? a.kb : room / tiles, smem);
   CUtensorMap ta, tx;
-  int rc = prism_get_tensor_map(c.a, (unsigned long long)c.terms.slots * a.all_panels * 16, (unsigned long long)c.K, (unsigned long long)c.K, 16, &ta);
+  int rc = prism_get_tensor_map(c.a, (unsigned long long)c.terms.slots * a.all_panels * 16, (unsigned long long)c.K, (unsigned long long)c.K, 16 * a.run, &ta);
   if (!rc) rc = prism_get_tensor_map(c.x, (unsigned long long)c.T, (unsigned long long)c.K, (unsigned long long)c.ldx, 128, &tx);
   if (rc) return rc;
   return (int)prism_launch_clusters(adapter_low_prompt_kernel, dim3(1, tiles, cs), dim3(TC_THREADS), smem, c.stream, c.pdl, cs, ta, tx, a);
@@ -1115,7 +1130,7 @@ PRISM_API int prism_adapter_linear(const void* x, const void* w, const void* a, 
                                    const void* lists, const void* counts, const void* bias, void* out, void* h, int T, int M, int K, int slots,
                                    int panels, int sections, const void* ends, int capacity, int tile_rows, int act, long long ldx, long long ldw,
                                    long long ldo, void* stream, int pdl) {
-  if (T < 1 || M < 1 || K < 1 || K % 8 || slots < 1 || panels < 1 || sections < 1 || sections > MAX_SECTIONS || capacity < 1) return -1;
+  if (T < 1 || M < 1 || K < 1 || K % 8 || slots < 1 || panels < 1 || sections < 1 || sections > MAX_SECTIONS || capacity < 1 || capacity > PLAN_TILE) return -1;
   if (act && (M % 2 || sections != 2 || bias != nullptr)) return -2;
   const int bn = T <= 16 ? 16 : T <= 32 ? 32 : T <= 64 ? 64 : 128;
   if (tile_rows != (T <= 128 ? bn : PLAN_TILE)) return -3;

@@ -19,6 +19,7 @@ namespace {
 constexpr int MAP_THREADS = 256;
 constexpr int MAP_WARPS = MAP_THREADS / 32;
 constexpr int MAP_MAX_REQUESTS = 8192;   // 12 bytes of shared memory each
+constexpr int MAP_MAX_ROWS = 1 << 30;     // tokens, and entries of a table row: strides stay inside 31 bits
 constexpr int MAP_SEGMENT = 128;         // entries of a table row that a warp writes at a time
 
 struct MapArgs {
@@ -190,7 +191,7 @@ PRISM_API int prism_step_maps(const void* pages, const void* page_offsets, const
                               const void* adapter, int S, int T, int W, int page, int n_pages, void* tables, void* slots, void* positions,
                               void* token_seq, void* token_adapter, void* cu_q, void* cu_kv, void* kv_lens, void* sample_rows,
                               void* stream, int pdl) {
-  if (S < 0 || S > MAP_MAX_REQUESTS || T < 0 || W < 1 || page < 1 || n_pages < 0) return -1;
+  if (S < 0 || S > MAP_MAX_REQUESTS || T < 0 || T > MAP_MAX_ROWS || W < 1 || W > MAP_MAX_ROWS || page < 1 || n_pages < 0) return -1;
   MapArgs a;
   a.pages = (const int*)pages;
   a.page_offsets = (const int*)page_offsets;

@@ -9,6 +9,7 @@ import torch
 sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
 from op_helpers import CPU, GPU16, GPU32, rand  # noqa: E402
 
+from prism_infer_b200 import ops  # noqa: E402
 from prism_infer_b200.ops import adapters, native  # noqa: E402
 
 BACKENDS = [CPU, GPU32, GPU16]
@@ -215,6 +216,84 @@ def test_calls_on_two_streams_at_once(backend):
         assert all(torch.equal(g, want[i]) for g in got[i])
 
 
+@pytest.mark.parametrize("backend", GPU)
+@pytest.mark.parametrize("T", [40, 300])
+def test_one_pool_on_two_streams_at_once(backend, T):
+    p, q = (Problem(backend, T, 512, (256,), 16, 8, mixed(T, 8), seed=3, scale=s) for s in (1.0, 2.0))
+    q.pool = p.pool
+    want = p.run().clone(), q.run().clone()
+    torch.cuda.synchronize()
+    streams, got = (torch.cuda.Stream(), torch.cuda.Stream()), ([], [])
+    for _ in range(10):
+        for i, r in enumerate((p, q)):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(r.run())
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, want[i]) for i in range(2) for g in got[i])
+
+
+@pytest.mark.parametrize("backend", GPU)
+@pytest.mark.parametrize("T", [12, 128, 300])
+def test_overlapped_launches_agree(backend, T):
+    """Programmatic launches of every kernel: the plan, two projections that read one another's results, bit for bit."""
+    p = Problem(backend, T, 256, (256,), 16, 6, mixed(T, 6))
+    x, w, who = p.to(p.x), p.to(p.w), p.who.to(p.device)
+
+    def chain():
+        y = x
+        for _ in range(6):
+            y = adapters.linear(y, w, p.pool, adapters.plan(who, 6)) * 0.5
+            y = adapters.linear(y, w, p.pool, adapters.plan(who, 6))
+        return y
+
+    want = chain().clone()
+    ops.set_pdl(True)
+    try:
+        got = [chain() for _ in range(5)]
+    finally:
+        ops.set_pdl(False)
+    assert all(torch.equal(g, want) for g in got)
+    native.check_status()
+
+
+@pytest.mark.parametrize("backend", BACKENDS)
+@pytest.mark.parametrize("T", [3, 40, 200])
+def test_large_ranks_and_all_sections(backend, T):
+    p = Problem(backend, T, 192, (24, 8, 40, 16, 32, 8, 64, 16), 40, 3, mixed(T, 3))
+    p.check(p.run())
+    p = Problem(backend, T, 64, (48, 48), 250, 3, mixed(T, 3), scale=0.25)
+    p.check(p.run())
+
+
+@pytest.mark.parametrize("backend", GPU)
+@pytest.mark.parametrize("T", [257, 300, 640, 1000])
+def test_steps_that_run_in_pieces(backend, T, monkeypatch):
+    """Low-rank rows that would pass their limit: a tile at a time, with bits as in one launch where the pieces' kernels are the same."""
+    p = Problem(backend, T, 128, (96, 32), 16, 40, mixed(T, 40), bias=True)
+    monkeypatch.setattr(adapters, "MAX_LOW_BYTES", 1)
+    out = torch.full((T, 160), 3.0, dtype=p.dtype, device=p.device)
+    p.check(p.run(out=out[:, 16:144]))
+    assert bool((out[:, :16] == 3.0).all()) and bool((out[:, 144:] == 3.0).all())
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda:0", marks=pytest.mark.gpu)])
+def test_odd_rows_in_32_bits(device):
+    """Widths and strides that no vector load fits."""
+    for T in (5, 70):
+        p = Problem((device, torch.float32), T, 37, (13, 6), 3, 4, mixed(T, 4), bias=True)
+        wide = torch.full((T, 39), 7.0, device=device)
+        wide[:, 1:38] = p.to(p.x)
+        p.check(adapters.linear(wide[:, 1:38], p.to(p.w), p.pool, p.plan, bias=p.to(p.bias)))
+
+
+@pytest.mark.parametrize("backend", BACKENDS)
+def test_factors_that_require_gradients_are_copied(backend):
+    p = Problem(backend, 4, 64, (32,), 8, 2, [0, 1, -1, 0])
+    a, b = torch.randn(8, 64, requires_grad=True), torch.randn(32, 8, requires_grad=True)
+    p.pool.load(1, a, b)
+    assert not p.pool.a.requires_grad and not p.run().requires_grad
+
+
 def plan_of(who, slots):
     index, lists, counts = [], [], []
     for lo in range(0, len(who), 256):
@@ -294,6 +373,7 @@ def test_refusals(backend):
     refused(pool.load, 0, a, b, float("nan"))
     refused(pool.load, 0, a, b * float("inf"))
     refused(pool.load, 0, a * 1e39, b)
+    refused(pool.load, 0, a, b, 1e39)
     refused(pool.clear, -1)
     if device == "cpu":
         refused(adapters.plan, torch.tensor([2], dtype=torch.int32), 2)

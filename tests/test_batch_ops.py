@@ -164,7 +164,7 @@ def test_refusals(backend):
     refused(i([[1]]), i([0]), i([1]), **ok)
     refused(i([1, 2, 3])[::2], i([0]), i([1]), **ok)
     refused(i([1]), i(0), i(1), **ok)
-    for bad in (dict(page=0), dict(width=0), dict(tokens=-1), dict(page=2 ** 31)):
+    for bad in (dict(page=0), dict(width=0), dict(tokens=-1), dict(page=2 ** 31), dict(tokens=2 ** 30 + 1), dict(width=2 ** 30 + 1)):
         refused(i([1]), i([0]), i([1]), **{**ok, **bad})
     for bad in (dict(page_offsets=i([0])), dict(shift=i([0, 0])), dict(adapter=i([0]).long())):
         refused(i([1]), i([0]), i([1]), **ok, **bad)
