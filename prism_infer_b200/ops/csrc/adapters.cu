@@ -684,17 +684,20 @@ struct LowF32Args {
   const float* scale;   // [slots]
   const int* adapter;   // [T]
   float* h;             // [T][low]; rows of tokens without an adapter are not written
-  int K, low, slots, vec;
+  int K, low, slots;
   long long ldx;
 };
 
-// Four consecutive values, zeros behind the end.
-__device__ __forceinline__ float4 load4(const float* p, int k, int K, bool vec) {
-  if (vec && k + 4 <= K) return *reinterpret_cast<const float4*>(p + k);
+// Four consecutive values, zeros behind the end.  VEC: rows are whole 16-byte vectors, and the load is a single predicated one; with a branch
+// around it loads waited for one another.
+template <bool VEC>
+__device__ __forceinline__ float4 load4(const float* p, int k, int K) {
+  if (VEC) return k < K ? __ldg(reinterpret_cast<const float4*>(p + k)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   return make_float4(k < K ? p[k] : 0.0f, k + 1 < K ? p[k + 1] : 0.0f, k + 2 < K ? p[k + 2] : 0.0f, k + 3 < K ? p[k + 3] : 0.0f);
 }
 
 // A warp per two rows of A, whose sums it keeps in four parts per lane.
+template <bool VEC>
 __global__ void __launch_bounds__(256) adapter_low_f32_kernel(const LowF32Args a) {
   const int t = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   pdl_wait();
@@ -706,11 +709,19 @@ __global__ void __launch_bounds__(256) adapter_low_f32_kernel(const LowF32Args a
   for (int r = (blockIdx.y * 8 + warp) * 2; r < a.low; r += gridDim.y * 16) {
     const float* const row = a.a + ((size_t)who * a.low + r) * a.K;
     float4 s0 = make_float4(0, 0, 0, 0), s1 = s0;
-#pragma unroll 4
-    for (int k = lane * 4; k < a.K; k += 128) {
-      const float4 v = load4(x, k, a.K, a.vec), p = load4(row, k, a.K, a.vec), q = load4(row + a.K, k, a.K, a.vec);
-      s0 = make_float4(fmaf(v.x, p.x, s0.x), fmaf(v.y, p.y, s0.y), fmaf(v.z, p.z, s0.z), fmaf(v.w, p.w, s0.w));
-      s1 = make_float4(fmaf(v.x, q.x, s1.x), fmaf(v.y, q.y, s1.y), fmaf(v.z, q.z, s1.z), fmaf(v.w, q.w, s1.w));
+    for (int k0 = lane * 4; k0 < a.K; k0 += 4 * 128) {   // twelve loads under way at a time
+      float4 v[4], p[4], q[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v[i] = load4<VEC>(x, k0 + i * 128, a.K);
+        p[i] = load4<VEC>(row, k0 + i * 128, a.K);
+        q[i] = load4<VEC>(row + a.K, k0 + i * 128, a.K);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        s0 = make_float4(fmaf(v[i].x, p[i].x, s0.x), fmaf(v[i].y, p[i].y, s0.y), fmaf(v[i].z, p[i].z, s0.z), fmaf(v[i].w, p[i].w, s0.w));
+        s1 = make_float4(fmaf(v[i].x, q[i].x, s1.x), fmaf(v[i].y, q[i].y, s1.y), fmaf(v[i].z, q[i].z, s1.z), fmaf(v[i].w, q[i].w, s1.w));
+      }
     }
     const float u = warp_sum((s0.x + s0.y) + (s0.z + s0.w)), w = warp_sum((s1.x + s1.y) + (s1.z + s1.w));
     if (lane < 2) a.h[(size_t)t * a.low + r + lane] = (lane ? w : u) * scale;
@@ -725,7 +736,7 @@ struct TileF32Args {
   const float* bias;    // [M] (null: none)
   const int* adapter;   // [T]
   float* out;           // [T][ldo]
-  int T, M, K, low, panels, slots, b_rows, vec, act;
+  int T, M, K, low, panels, slots, b_rows, act;
   long long ldx, ldw, ldo;
   int sections;
   int end[MAX_SECTIONS], shift[MAX_SECTIONS];   // shift: of a section's features in b
@@ -752,51 +763,61 @@ __device__ __forceinline__ float low_term(const TileF32Args& a, const float* h, 
   return sum;
 }
 
-constexpr int F32_THREADS = 128, F32_K = 32, F32_FOLD = 4;   // F32_FOLD chunks of F32_K products per accumulator
+constexpr int F32_THREADS = 128, F32_SUM = 128;   // F32_SUM products per accumulator
+__host__ __device__ constexpr int f32_chunk(int nt) { return nt == 2 ? 64 : 16; }   // columns of a chunk: few tokens are bound by the weights under way
 
-template <int NT, bool DUAL>
-__global__ void __launch_bounds__(F32_THREADS, 4) adapter_gemm_f32_kernel(const TileF32Args a) {
-  constexpr int TN = 8 * NT, WP = 68, XP = TN + 4, LOADS = TN * F32_K / 4 / F32_THREADS, QUADS = DUAL ? 8 : 16, RED = 68;
-  __shared__ __align__(16) float ws[2][F32_K][WP];
-  __shared__ __align__(16) float xs[2][F32_K][XP];
-  static_assert(TN * RED <= 2 * F32_K * WP, "the sums take the weights' place");
-  float* const red = &ws[0][0][0];
+// A thread sums NF of the tile's 64 features for NT tokens.  8 x 8 from 65 tokens: 4 loads of 16 bytes from shared memory feed 64 multiply-adds,
+// where 4 x 8 was bound by these loads (300 tokens, 2048 -> 4096: 297 us with 4 x 8, 196 us with 8 x 8 though a quarter of its tokens is
+// padding; 700 tokens, 4096 -> 4096: 689 us, 34 TFLOP/s).  Chunks are stored k by k; runs of features or tokens change places with k / 4, which
+// keeps stores and loads clear of bank conflicts (1.6 million of them in 0.54 million stores without).
+template <int NF, int NT, bool DUAL, bool VEC>
+__global__ void __launch_bounds__(F32_THREADS, NF == 8 ? 3 : 4) adapter_gemm_f32_kernel(const TileF32Args a) {
+  constexpr int KC = f32_chunk(NT), QUADS_K = KC / 4, ROWS = F32_THREADS / QUADS_K, FOLD = F32_SUM / KC;
+  constexpr int FX = 64 / NF, TG = F32_THREADS / FX, TN = TG * NT;   // threads side by side over the features, groups of tokens
+  constexpr int WP = 68, XP = TN + 4, W_LOADS = 64 / ROWS, LOADS = (TN + ROWS - 1) / ROWS, QUADS = DUAL ? 8 : 16, RED = 68;
+  extern __shared__ float4 smem_f32[];
+  float* const smem = reinterpret_cast<float*>(smem_f32);
+  float (*const ws)[KC][WP] = reinterpret_cast<float (*)[KC][WP]>(smem);
+  float (*const xs)[KC][XP] = reinterpret_cast<float (*)[KC][XP]>(smem + 2 * KC * WP);
+  float* const red = smem + 2 * KC * (WP + XP);   // the sums so far: registers hold those of the last chunks only
   const int cs = gridDim.z, z = blockIdx.z, tid = threadIdx.x;
   const int f0 = blockIdx.x * (DUAL ? 32 : 64), t0 = blockIdx.y * TN, half = a.M / 2;
-  const int chunks = (a.K + F32_K - 1) / F32_K, c0 = part_begin(chunks, z, cs), c1 = part_begin(chunks, z + 1, cs);
+  const int chunks = (a.K + KC - 1) / KC, c0 = part_begin(chunks, z, cs), c1 = part_begin(chunks, z + 1, cs);
+  const int quad = tid % QUADS_K, line = tid / QUADS_K;   // the four columns of a chunk and the rows that this thread copies
+  auto turn_of = [](int q) { return KC == 16 ? q << 3 : (q & 7) << 2; };
   // row i of the weight tile; a row outside the matrix reads as zeros
   auto w_row = [&](int i) { return DUAL ? (i < 32 ? (f0 + i < half ? f0 + i : -1) : (f0 + i - 32 < half ? half + f0 + i - 32 : -1)) : (f0 + i < a.M ? f0 + i : -1); };
-  float4 wr[4], xr[LOADS];
+  float4 wr[W_LOADS], xr[LOADS];
   auto fetch = [&](int chunk) {
-    const int k = chunk * F32_K + (tid & 7) * 4;
+    const int k = chunk * KC + quad * 4;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int r = w_row((tid >> 3) + i * 16);
-      wr[i] = r < 0 ? make_float4(0, 0, 0, 0) : load4(a.w + (size_t)r * a.ldw, k, a.K, a.vec);
+    for (int i = 0; i < W_LOADS; ++i) {
+      const int r = w_row(line + i * ROWS);
+      wr[i] = r < 0 ? make_float4(0, 0, 0, 0) : load4<VEC>(a.w + (size_t)r * a.ldw, k, a.K);
     }
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
-      const int t = t0 + (tid >> 3) + i * 16;
-      xr[i] = t < a.T ? load4(a.x + (size_t)t * a.ldx, k, a.K, a.vec) : make_float4(0, 0, 0, 0);
+      const int c = line + i * ROWS;
+      xr[i] = c < TN && t0 + c < a.T ? load4<VEC>(a.x + (size_t)(t0 + c) * a.ldx, k, a.K) : make_float4(0, 0, 0, 0);
     }
   };
-  // Turned: k by k.  Rows change places with k / 4, which spreads the stores over the banks (without, 1.6 million conflicts in 0.54 million
-  // stores for 100 tokens, 2048 -> 2048).
   auto keep = [&](int buf) {
-    const int k = (tid & 7) * 4;
+    const int k = quad * 4;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int r = ((tid >> 3) + i * 16) ^ k;
+    for (int i = 0; i < W_LOADS; ++i) {
+      const int r = (line + i * ROWS) ^ turn_of(quad);
       ws[buf][k][r] = wr[i].x, ws[buf][k + 1][r] = wr[i].y, ws[buf][k + 2][r] = wr[i].z, ws[buf][k + 3][r] = wr[i].w;
     }
 #pragma unroll
-    for (int i = 0; i < LOADS; ++i) {
-      const int r = ((tid >> 3) + i * 16) ^ (k & (TN - 1));
-      xs[buf][k][r] = xr[i].x, xs[buf][k + 1][r] = xr[i].y, xs[buf][k + 2][r] = xr[i].z, xs[buf][k + 3][r] = xr[i].w;
-    }
+    for (int i = 0; i < LOADS; ++i)
+      if (line + i * ROWS < TN) {
+        const int r = (line + i * ROWS) ^ (turn_of(quad) & (TN - 1));
+        xs[buf][k][r] = xr[i].x, xs[buf][k + 1][r] = xr[i].y, xs[buf][k + 2][r] = xr[i].z, xs[buf][k + 3][r] = xr[i].w;
+      }
   };
-  const int fx = (tid & 15) * 4, tx = (tid >> 4) * NT;   // this thread's 4 features and NT tokens
-  float acc[NT][4] = {}, total[NT][4] = {};
+  // this thread's features fx .. + 4 (and 32 further on) and tokens tx .. + 4 (and TG * 4 further on; NT 2: tx .. + 2)
+  const int fx = (tid % FX) * 4, tx = (tid / FX) * (NT < 4 ? NT : 4);
+  float acc[NT][NF] = {};
   pdl_launch_dependents();
   fetch(c0);
   keep(0);
@@ -805,30 +826,37 @@ __global__ void __launch_bounds__(F32_THREADS, 4) adapter_gemm_f32_kernel(const 
     const int buf = (c - c0) & 1;
     if (c + 1 < c1) fetch(c + 1);
 #pragma unroll
-    for (int k = 0; k < F32_K; ++k) {
-      const float4 w = *reinterpret_cast<const float4*>(&ws[buf][k][fx ^ (k & ~3)]);
-      float x[NT];
+    for (int k = 0; k < KC; ++k) {
+      const int turn = turn_of(k >> 2);
+      float w[NF], x[NT];
 #pragma unroll
-      for (int i = 0; i < NT; i += 2) *reinterpret_cast<float2*>(&x[i]) = *reinterpret_cast<const float2*>(&xs[buf][k][(tx + i) ^ (k & ~3 & (TN - 1))]);
+      for (int e = 0; e < NF; e += 4) *reinterpret_cast<float4*>(&w[e]) = *reinterpret_cast<const float4*>(&ws[buf][k][(fx + e * 8) ^ turn]);
+      if (NT < 4) {
+        *reinterpret_cast<float2*>(x) = *reinterpret_cast<const float2*>(&xs[buf][k][tx ^ (turn & (TN - 1))]);
+      } else {
 #pragma unroll
-      for (int i = 0; i < NT; ++i) {
-        acc[i][0] = fmaf(x[i], w.x, acc[i][0]);
-        acc[i][1] = fmaf(x[i], w.y, acc[i][1]);
-        acc[i][2] = fmaf(x[i], w.z, acc[i][2]);
-        acc[i][3] = fmaf(x[i], w.w, acc[i][3]);
+        for (int i = 0; i < NT; i += 4) *reinterpret_cast<float4*>(&x[i]) = *reinterpret_cast<const float4*>(&xs[buf][k][(tx + i * TG) ^ turn]);
       }
-    }
-    if ((c - c0) % F32_FOLD == F32_FOLD - 1 || c + 1 == c1) {
 #pragma unroll
       for (int i = 0; i < NT; ++i)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) total[i][e] += acc[i][e], acc[i][e] = 0.0f;
+        for (int e = 0; e < NF; ++e) acc[i][e] = fmaf(x[i], w[e], acc[i][e]);
+    }
+    if ((c - c0) % FOLD == FOLD - 1 || c + 1 == c1) {
+#pragma unroll
+      for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int e = 0; e < NF; e += 4) {
+          float4* const sum = reinterpret_cast<float4*>(&red[(NT < 4 ? tx + i : tx + (i & 3) + (i >> 2) * 4 * TG) * RED + fx + e * 8]);
+          float4 v = make_float4(acc[i][e], acc[i][e + 1], acc[i][e + 2], acc[i][e + 3]);
+          if (c - c0 >= FOLD) v = add4(*sum, v);
+          *sum = v;
+          acc[i][e] = acc[i][e + 1] = acc[i][e + 2] = acc[i][e + 3] = 0.0f;
+        }
     }
     if (c + 1 < c1) keep(buf ^ 1);
     __syncthreads();
   }
-#pragma unroll
-  for (int i = 0; i < NT; ++i) *reinterpret_cast<float4*>(&red[(tx + i) * RED + fx]) = make_float4(total[i][0], total[i][1], total[i][2], total[i][3]);
   pdl_wait();   // the low-rank rows
   cluster_sync_all();
   const int items = min(TN, a.T - t0) * QUADS;
@@ -1088,14 +1116,34 @@ PRISM_API int prism_adapter_plan(const void* adapter, int T, int slots, int capa
 
 namespace {
 
-template <int NT, bool DUAL>
-int launch_f32(const TileF32Args& a, cudaStream_t stream) {
+template <int NF, int NT, bool DUAL, bool VEC>
+int launch_f32_tiles(const TileF32Args& a, cudaStream_t stream) {
+  static std::atomic<unsigned long long> devices{0};
   static ClusterTable table;
-  const long long tiles = (long long)((DUAL ? a.M / 2 + 31 : a.M + 63) / (DUAL ? 32 : 64)) * ((a.T + 8 * NT - 1) / (8 * NT));
-  const int chunks = (a.K + F32_K - 1) / F32_K;
-  const int cs = cluster_size(table, tiles, chunks / F32_FOLD, 56 * 1024);   // four blocks per SM, at least 128 products each
-  const dim3 grid((unsigned)((DUAL ? a.M / 2 + 31 : a.M + 63) / (DUAL ? 32 : 64)), (unsigned)((a.T + 8 * NT - 1) / (8 * NT)), cs);
-  return (int)prism_launch_clusters(adapter_gemm_f32_kernel<NT, DUAL>, grid, dim3(F32_THREADS), 0, stream, true, cs, a);
+  constexpr int TN = F32_THREADS / (64 / NF) * NT;
+  constexpr int KC = f32_chunk(NT);
+  const size_t smem = (size_t)(2 * KC * (68 + TN + 4) + TN * 68) * sizeof(float);
+  const cudaError_t e = allow_smem(adapter_gemm_f32_kernel<NF, NT, DUAL, VEC>, devices);
+  if (e != cudaSuccess) return (int)e;
+  const int f_tiles = DUAL ? (a.M / 2 + 31) / 32 : (a.M + 63) / 64, t_tiles = (a.T + TN - 1) / TN, most = a.K / F32_SUM;
+  // At least 128 products a block.  What counts is the SM with the most blocks, each a share of K; one block alone, four warps, keeps an SM little
+  // more than half as busy as three do (300 tokens, 2048 -> 4096, 192 tiles: 376 us, in clusters of two 196).
+  const long long tiles = (long long)f_tiles * t_tiles;
+  int cs = 1;
+  double best = 0.0;
+  for (int n = 1; n <= 8 && n <= (most < 1 ? 1 : most); n *= 2) {
+    const long long blocks = (tiles * n + SMS - 1) / SMS;
+    if (n > 1 && (blocks > 3 || cluster_size(table, tiles, n, 64 * 1024) != n)) break;
+    const double cost = (double)blocks / n * (blocks == 1 ? 1.7 : blocks == 2 ? 1.2 : 1.0);
+    if (n == 1 || cost <= best) cs = n, best = cost;
+  }
+  return (int)prism_launch_clusters(adapter_gemm_f32_kernel<NF, NT, DUAL, VEC>, dim3(f_tiles, t_tiles, cs), dim3(F32_THREADS), smem, stream, true, cs, a);
+}
+
+template <int NF, int NT>
+int launch_f32(const TileF32Args& a, bool vec, cudaStream_t on) {
+  if (vec) return a.act ? launch_f32_tiles<NF, NT, true, true>(a, on) : launch_f32_tiles<NF, NT, false, true>(a, on);
+  return a.act ? launch_f32_tiles<NF, NT, true, false>(a, on) : launch_f32_tiles<NF, NT, false, false>(a, on);
 }
 
 }  // namespace
@@ -1104,24 +1152,26 @@ int launch_f32(const TileF32Args& a, cudaStream_t stream) {
 PRISM_API int prism_adapter_linear_f32(const void* x, const void* w, const void* a, const void* b, const void* scale, const void* adapter,
                                        const void* bias, void* out, void* h, int T, int M, int K, int slots, int panels, int sections, const void* ends,
                                        int act, long long ldx, long long ldw, long long ldo, void* stream, int pdl) {
-  if (T < 1 || T > 65535 * 16 || M < 1 || K < 1 || slots < 1 || panels < 1 || sections < 1 || sections > MAX_SECTIONS) return -1;
+  if (T < 1 || T > 65535 * 64 || M < 1 || K < 1 || slots < 1 || panels < 1 || sections < 1 || sections > MAX_SECTIONS) return -1;
   if (act && (M % 2 || sections != 2 || bias != nullptr)) return -2;
   const bool vec = (((uintptr_t)x | (uintptr_t)w | (uintptr_t)a) & 15) == 0 && K % 4 == 0 && ldx % 4 == 0 && ldw % 4 == 0;
   const int low = sections * panels * 16;
-  LowF32Args l{(const float*)x, (const float*)a, (const float*)scale, (const int*)adapter, (float*)h, K, low, slots, vec, ldx};
+  LowF32Args l{(const float*)x, (const float*)a, (const float*)scale, (const int*)adapter, (float*)h, K, low, slots, ldx};
   // few tokens: a block per 16 rows
-  const cudaError_t e = prism_launch(adapter_low_f32_kernel, dim3(T, T < 148 ? (low + 15) / 16 : 1), dim3(256), 0, (cudaStream_t)stream, pdl != 0, l);
+  const cudaError_t e = prism_launch(vec ? adapter_low_f32_kernel<true> : adapter_low_f32_kernel<false>, dim3(T, T < 148 ? (low + 15) / 16 : 1), dim3(256), 0, (cudaStream_t)stream, pdl != 0, l);
   if (e != cudaSuccess) return (int)e;
   TileF32Args t{(const float*)x, (const float*)w, (const float*)b, (const float*)h, (const float*)bias, (const int*)adapter, (float*)out,
-                T, M, K, low, panels, slots, 0, vec, act, ldx, ldw, ldo, sections, {}, {}};
+                T, M, K, low, panels, slots, 0, act, ldx, ldw, ldo, sections, {}, {}};
   for (int s = 0; s < sections; ++s) {
     const int start = s ? t.end[s - 1] : 0;
     t.end[s] = ((const int*)ends)[s];
     t.shift[s] = t.b_rows - start;
     t.b_rows += (t.end[s] - start + 7) / 8 * 8;
   }
-  if (T <= 16) return act ? launch_f32<2, true>(t, (cudaStream_t)stream) : launch_f32<2, false>(t, (cudaStream_t)stream);
-  return act ? launch_f32<8, true>(t, (cudaStream_t)stream) : launch_f32<8, false>(t, (cudaStream_t)stream);
+  cudaStream_t on = (cudaStream_t)stream;
+  if (T <= 16) return launch_f32<4, 2>(t, vec, on);
+  if (T <= 64) return launch_f32<4, 8>(t, vec, on);
+  return launch_f32<8, 8>(t, vec, on);
 }
 
 // bf16 projection (act 0) or gated unit (PRISM_GLU_*) with the adapters of a plan.  lists, counts: of the call's tiles of 256 tokens;
