@@ -158,20 +158,21 @@ def _ld(t: torch.Tensor) -> int:
 
 def _check(x: torch.Tensor, w: torch.Tensor, pool: AdapterPool, p: AdapterPlan, bias: Optional[torch.Tensor], out: Optional[torch.Tensor],
            features: int) -> None:
-    if x.dim() != 2 or w.dim() != 2 or x.shape[1] != pool.in_features or tuple(w.shape) != (pool.features, pool.in_features):
-        raise ValueError(f"x {tuple(x.shape)} and w {tuple(w.shape)} for a pool of {pool.in_features} -> {pool.features}")
-    tensors = [x, w] + [t for t in (bias, out) if t is not None]
-    if any(t.dtype != pool.dtype or t.device != pool.device for t in tensors) or p.adapter.device != pool.device:
-        raise ValueError(f"tensors must be {pool.dtype} on {pool.device}, as the pool is")
+    dtype, device, K = pool.dtype, pool.device, pool.in_features
+    if x.dim() != 2 or w.dim() != 2 or x.shape[1] != K or w.shape[0] != pool.features or w.shape[1] != K:
+        raise ValueError(f"x {tuple(x.shape)} and w {tuple(w.shape)} for a pool of {K} -> {pool.features}")
+    if x.dtype != dtype or w.dtype != dtype or x.device != device or w.device != device or p.adapter.device != device:
+        raise ValueError(f"tensors must be {dtype} on {device}, as the pool is")
     if p.slots != pool.slots or p.adapter.shape[0] != x.shape[0]:
         raise ValueError(f"a plan of {p.adapter.shape[0]} tokens over {p.slots} slots for {x.shape[0]} tokens and {pool.slots} slots")
-    if bias is not None and (tuple(bias.shape) != (pool.features,) or not bias.is_contiguous()):
-        raise ValueError(f"bias must be contiguous, one value for each of {pool.features} features")
-    if out is not None and (tuple(out.shape) != (x.shape[0], features) or (features > 1 and out.stride(1) != 1) or _ld(out) < features):
-        raise ValueError(f"out must have shape {(x.shape[0], features)} and contiguous rows that are apart")
+    if bias is not None and (bias.dtype != dtype or bias.device != device or bias.shape != (pool.features,) or not bias.is_contiguous()):
+        raise ValueError(f"bias must be contiguous {dtype} on {device}, one value for each of {pool.features} features")
+    if out is not None and (out.dtype != dtype or out.device != device or out.shape != (x.shape[0], features) or (features > 1 and out.stride(1) != 1)
+                            or _ld(out) < features):
+        raise ValueError(f"out must be {dtype} on {device} of shape {(x.shape[0], features)}, with contiguous rows that are apart")
     for name, t in (("x", x), ("w", w)):
         ld = _ld(t)
-        if t.stride(1) != 1 or ld < t.shape[1] or (t.dtype == torch.bfloat16 and (ld % 8 or t.data_ptr() % 16)):
+        if t.stride(1) != 1 or ld < K or (dtype == torch.bfloat16 and (ld % 8 or t.data_ptr() % 16)):
             raise ValueError(f"{name}: rows must be contiguous and apart, in bf16 on 16-byte boundaries")
     check_device(x)
 

@@ -1076,8 +1076,8 @@ int launch_tiles(const Call& c) {
   CUtensorMap tw, tx, tb, th;
   int rc = prism_get_tensor_map(c.w, (unsigned long long)c.M, (unsigned long long)c.K, (unsigned long long)c.ldw, FEATURES, &tw);
   if (!rc) rc = prism_get_tensor_map(c.x, (unsigned long long)c.T, (unsigned long long)c.K, (unsigned long long)c.ldx, BN, &tx);
-  if (!rc) rc = prism_make_panel_tensor_map(c.b, (unsigned long long)a.no_group, FEATURES / 8, &tb);
-  if (!rc) rc = prism_make_panel_tensor_map(c.h, (unsigned long long)t.tiles * t.capacity * all * c.tile_rows / 8, BN / 8, &th);
+  if (!rc) rc = prism_get_panel_tensor_map(c.b, (unsigned long long)a.no_group, FEATURES / 8, &tb);
+  if (!rc) rc = prism_get_panel_tensor_map(c.h, (unsigned long long)t.tiles * t.capacity * all * c.tile_rows / 8, BN / 8, &th);
   if (rc) return rc;
   return (int)prism_launch_clusters(adapter_gemm_kernel<BN, DUAL>, dim3(m_tiles, token_tiles, cs), dim3(TC_THREADS), smem, c.stream, true, cs, tw, tx, tb,
                                     th, a);

@@ -413,8 +413,8 @@ int prism_get_tensor_map(const void* ptr, unsigned long long rows, unsigned long
 int prism_make_head_tensor_map(const void* ptr, unsigned long long tokens, unsigned heads, unsigned head_dim,
                                unsigned long long ld, unsigned box_rows, CUtensorMap* out);
 // Panels of 16 ranks in memory as the MMA reads them: groups of 8 rows, each [2][8 rows][8 ranks] bf16 = 256 bytes.  A copy moves box_groups
-// groups; 256-byte rows of the copy engine (as [rows][16] with 32-byte rows, a panel of 128 rows took it some 0.2 us).  Not cached.
-int prism_make_panel_tensor_map(const void* ptr, unsigned long long groups, unsigned box_groups, CUtensorMap* out);
+// groups; 256-byte rows of the copy engine (as [rows][16] with 32-byte rows, eight panels of 128 rows took it some 2 us).  Cached as above.
+int prism_get_panel_tensor_map(const void* ptr, unsigned long long groups, unsigned box_groups, CUtensorMap* out);
 // Prompt products with low-rank adapters on SM pairs (gemm_pair.cuh), as adapters.cu describes them.
 struct PrismAdapterSections {
   int n;            // sections of the stacked matrix

@@ -915,7 +915,14 @@ int prism_make_head_tensor_map(const void* ptr, unsigned long long tokens, unsig
   return r == CUDA_SUCCESS ? 0 : -102 - (int)r;
 }
 
-int prism_make_panel_tensor_map(const void* ptr, unsigned long long groups, unsigned box_groups, CUtensorMap* out) {
+int prism_get_panel_tensor_map(const void* ptr, unsigned long long groups, unsigned box_groups, CUtensorMap* out) {
+  const MapKey key{ptr, groups, 0, 0, box_groups};   // no matrix has rows of no columns
+  std::lock_guard<std::mutex> lock(g_map_mutex);
+  auto it = g_maps.find(key);
+  if (it != g_maps.end()) {
+    *out = it->second;
+    return 0;
+  }
   EncodeTiledFn fn = get_encode_fn();
   if (!fn) return -100;
   if (reinterpret_cast<uintptr_t>(ptr) & 15) return -101;
@@ -926,7 +933,10 @@ int prism_make_panel_tensor_map(const void* ptr, unsigned long long groups, unsi
   CUresult r = fn(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(ptr), dims, strides, box, estr,
                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  return r == CUDA_SUCCESS ? 0 : -102 - (int)r;
+  if (r != CUDA_SUCCESS) return -102 - (int)r;
+  if (g_maps.size() > 65536) g_maps.clear();
+  g_maps.emplace(key, *out);
+  return 0;
 }
 
 // The pairs' epilogue moves whole 16-byte vectors of 16 features at a time, from the start of every section.
@@ -989,8 +999,8 @@ int prism_adapter_pair(const void* W, const void* X, void* out, int M, int T, in
   CUtensorMap tx, tw, th, tb;
   int rc = get_tensor_map(X, (unsigned long long)T, (unsigned long long)K, (unsigned long long)ldx, 128, &tx);
   if (!rc) rc = get_tensor_map(W, (unsigned long long)M, (unsigned long long)K, (unsigned long long)ldw, (unsigned)(a.bn / 2), &tw);
-  if (!rc) rc = prism_make_panel_tensor_map(t.h, (unsigned long long)t.tiles * t.capacity * d.all_panels * 32, 16, &th);
-  if (!rc) rc = prism_make_panel_tensor_map(t.b, (unsigned long long)d.no_group, (unsigned)(a.bn / 16), &tb);
+  if (!rc) rc = prism_get_panel_tensor_map(t.h, (unsigned long long)t.tiles * t.capacity * d.all_panels * 32, 16, &th);
+  if (!rc) rc = prism_get_panel_tensor_map(t.b, (unsigned long long)d.no_group, (unsigned)(a.bn / 16), &tb);
   if (rc) return rc;
   const cudaError_t e = cudaFuncSetAttribute(gemm_pair_adapter_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_LIMIT);
   if (e != cudaSuccess) return (int)e;
