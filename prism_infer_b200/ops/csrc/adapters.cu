@@ -533,24 +533,22 @@ adapter_gemm_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_consta
     tmem_alloc(tmem_slot, TMEM_COLS);
     tmem_relinquish();
   }
+  // The plan's kernel is done, but this one has not waited for it: list and count come from L2, past what an older kernel left in L1.
+  __shared__ int list[PLAN_TILE];
+  for (int j = (int)threadIdx.x - 64; j >= 0 && j < a.capacity; j += TC_THREADS - 64) list[j] = __ldcg(a.lists + (size_t)tile * a.capacity + j);
+  const int count = min(__ldcg(a.counts + tile), a.capacity);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   pdl_launch_dependents();
 
-  const int per = DUAL ? a.all_panels : a.panels;   // panels of one adapter that reach this tile
+  const int per = DUAL ? a.all_panels : a.panels, extra = count * per;   // panels of one adapter that reach this tile, and of all its adapters
   if (warp == 0) {
     if (elect_one()) {
-      const int extra = min(a.counts[tile], a.capacity) * per;
-      const int* const list = a.lists + (size_t)tile * a.capacity;
-      // this CTA's panels: adapter j of the list, panel rp of its section (of: of all sections), the slots asked for one adapter ahead
+      // this CTA's panels: adapter j of the list, panel rp of its section (of: of all sections)
       const int e_begin = part_begin(extra, z, cs), e_end = part_begin(extra, z + 1, cs), of0 = DUAL ? 0 : section * a.panels;
-      int j = e_begin / per, of = of0 + (e_begin - j * per), rp = of % a.panels, slot = 0, next = 0;
-      if (e_begin < e_end) {
-        slot = list[j];
-        next = list[min(j + 1, a.capacity - 1)];
-      }
+      int j = e_begin / per, of = of0 + (e_begin - j * per), rp = of % a.panels;
       const int b_at = DUAL ? f0 / 8 : a.b_start[section] + (f0 - a.start[section]) / 8;
       int s = 0;
       uint32_t parity = 1;   // a fresh empty barrier counts as free
@@ -573,7 +571,7 @@ adapter_gemm_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_consta
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           if (i < n) {
-            const int group = (slot * a.panels + rp) * a.b_groups + b_at;
+            const int group = (list[j] * a.panels + rp) * a.b_groups + b_at;
             if (DUAL) {   // a gate's panel adds nothing to the up half, and the other way round
               const bool up = of >= a.panels;
               tma_load_2d(st + i * 4096, &tmB, &full[s], 0, up ? a.no_group : group);
@@ -589,8 +587,6 @@ adapter_gemm_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_consta
               if (!DUAL || of == a.all_panels) {
                 of = of0;
                 ++j;
-                slot = next;
-                next = list[min(j + 1, a.capacity - 1)];
               }
             }
           }
@@ -607,7 +603,6 @@ adapter_gemm_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_consta
   } else if (warp == 1) {
     if (elect_one()) {
       constexpr uint32_t idesc = umma_idesc_bf16(128, BN);
-      const int extra = min(a.counts[tile], a.capacity) * per;
       int s = 0;
       uint32_t parity = 0;
       bool ok = true;
@@ -689,11 +684,13 @@ struct LowF32Args {
 };
 
 // Four consecutive values, zeros behind the end.  VEC: rows are whole 16-byte vectors, and the load is a single predicated one; with a branch
-// around it loads waited for one another.
+// around it loads waited for one another.  From L2: the projection starts before it has waited for the kernels whose results it reads here
+// (they are done), so nothing may come from a line that an older kernel left in L1.
 template <bool VEC>
 __device__ __forceinline__ float4 load4(const float* p, int k, int K) {
-  if (VEC) return k < K ? __ldg(reinterpret_cast<const float4*>(p + k)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  return make_float4(k < K ? p[k] : 0.0f, k + 1 < K ? p[k + 1] : 0.0f, k + 2 < K ? p[k + 2] : 0.0f, k + 3 < K ? p[k + 3] : 0.0f);
+  if (VEC) return k < K ? __ldcg(reinterpret_cast<const float4*>(p + k)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  return make_float4(k < K ? __ldcg(p + k) : 0.0f, k + 1 < K ? __ldcg(p + k + 1) : 0.0f, k + 2 < K ? __ldcg(p + k + 2) : 0.0f,
+                     k + 3 < K ? __ldcg(p + k + 3) : 0.0f);
 }
 
 // A warp per two rows of A, whose sums it keeps in four parts per lane.

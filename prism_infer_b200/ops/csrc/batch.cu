@@ -44,7 +44,7 @@ struct MapArgs {
 enum { MAP_LENGTH = 1, MAP_TOKENS = 2, MAP_WIDTH = 3, MAP_PAGES = 4 };   // details of a failed bounds check
 
 __device__ __forceinline__ int lengths_of(const MapArgs& a, int i, int& cached, int& fresh) {
-  const int c = __ldg(a.cached + i), f = __ldg(a.fresh + i);
+  const int c = __ldcg(a.cached + i), f = __ldcg(a.fresh + i);   // the step before may have written them on this SM
   const bool bad = c < 0 || f < 0 || c > 0x7fffffff - f;
   cached = bad ? 0 : c;
   fresh = bad ? 0 : f;

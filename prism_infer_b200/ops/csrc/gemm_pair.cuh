@@ -207,8 +207,9 @@ __device__ __forceinline__ void gemm_pair_body(const CUtensorMap& tmX, const CUt
     }
     return s;
   };
-  // panels of a token tile that reach a tile of features: of its section, or of the gate and the up half of a gated unit
-  auto panels_of = [&](int m0) { return min(d.counts[m0 / 256], d.capacity) * (a.dual ? d.all_panels : d.panels); };
+  // Panels of a token tile that reach a tile of features: of its section, or of the gate and the up half of a gated unit.  Counts and lists are
+  // read past L1: the kernel that made them is done, but this one has not waited for it.
+  auto panels_of = [&](int m0) { return min(__ldcg(d.counts + m0 / 256), d.capacity) * (a.dual ? d.all_panels : d.panels); };
 
   if (warp == 0) {
     if (elect_one()) {
@@ -236,8 +237,8 @@ __device__ __forceinline__ void gemm_pair_body(const CUtensorMap& tmX, const CUt
           extra = panels_of(m0);
           list = d.lists + (size_t)(m0 / 256) * d.capacity;
           if (extra > 0) {
-            slot = list[0];
-            next = list[min(1, d.capacity - 1)];
+            slot = __ldcg(list);
+            next = __ldcg(list + min(1, d.capacity - 1));
           }
         }
         for (int kb = kb0; kb < kb1; ++kb) {
@@ -276,7 +277,7 @@ __device__ __forceinline__ void gemm_pair_body(const CUtensorMap& tmX, const CUt
                     of = of0;
                     ++j;
                     slot = next;
-                    next = list[min(j + 1, d.capacity - 1)];
+                    next = __ldcg(list + min(j + 1, d.capacity - 1));
                   }
                 }
               }
