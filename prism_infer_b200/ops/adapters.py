@@ -195,26 +195,32 @@ def _adapted_cpu(x, w, pool, p, bias):
 MAX_LOW_BYTES = 256 << 20
 
 
+def _tile_rows(tokens: int) -> int:
+    """Tokens of a panel: those of a decode step, rounded up to the kernels' sizes, or a tile of a prompt."""
+    return TILE_TOKENS if tokens > 128 else 16 if tokens <= 16 else 1 << (tokens - 1).bit_length()
+
+
 def _run(x, w, pool, p, bias, out, act):
     T = x.shape[0]
     if T == 0:
         return out
     if pool.dtype == torch.float32:
         return _run_f32(x, w, pool, p, bias, out, act)
-    capacity, all_panels = p.lists.shape[1], pool.low // PANEL
-    tile_rows = TILE_TOKENS if T > 128 else max(16, 1 << (T - 1).bit_length())
-    per_tile = capacity * all_panels * tile_rows * PANEL     # values of every panel that a tile's adapters may need
-    tiles = p.lists.shape[0]
+    tiles, capacity = p.lists.shape
+    tile_rows, ldx, ldo = _tile_rows(T), _ld(x), _ld(out)
+    per_tile = capacity * pool.low * tile_rows     # values of every panel that a tile's adapters may need
     run = min(tiles, max(1, MAX_LOW_BYTES // (2 * per_tile)))
     h = torch.empty(run * per_tile, dtype=torch.bfloat16, device=x.device)
-    for first in range(0, tiles, run):
-        t0, n = first * TILE_TOKENS, min(run * TILE_TOKENS, T - first * TILE_TOKENS)
-        if tiles > run:
-            tile_rows = TILE_TOKENS if n > 128 else max(16, 1 << (n - 1).bit_length())
-        native.call("prism_adapter_linear", x.data_ptr() + 2 * t0 * _ld(x), _p(w), _p(pool.a), _p(pool.b), _p(pool.scale), p.index.data_ptr() + 4 * t0,
-                    p.lists.data_ptr() + 4 * first * capacity, p.counts.data_ptr() + 4 * first, _p(bias), out.data_ptr() + 2 * t0 * _ld(out), _p(h), n,
-                    pool.features, pool.in_features, pool.slots, pool.panels, len(pool.sections), pool._ends, capacity, tile_rows, act, _ld(x), _ld(w),
-                    _ld(out), _s(), _pdl())
+    x_at, out_at, index_at, lists_at, counts_at = x.data_ptr(), out.data_ptr(), p.index.data_ptr(), p.lists.data_ptr(), p.counts.data_ptr()
+    rest = (pool.features, pool.in_features, pool.slots, pool.panels, len(pool.sections), pool._ends, capacity)
+    n = min(run * TILE_TOKENS, T)
+    while T > 0:
+        if n > T:       # the last run of several
+            n, tile_rows = T, _tile_rows(T)
+        native.call("prism_adapter_linear", x_at, w.data_ptr(), pool.a.data_ptr(), pool.b.data_ptr(), pool.scale.data_ptr(), index_at, lists_at, counts_at,
+                    _p(bias), out_at, h.data_ptr(), n, *rest, tile_rows, act, ldx, _ld(w), ldo, _s(), _pdl())
+        x_at, out_at, index_at = x_at + 2 * n * ldx, out_at + 2 * n * ldo, index_at + 4 * n
+        lists_at, counts_at, T = lists_at + 4 * run * capacity, counts_at + 4 * run, T - n
     return out
 
 

@@ -41,7 +41,7 @@ class StepMaps:
 def _check_index(name: str, t: torch.Tensor, device: torch.device, shape: Optional[tuple[int, ...]] = None) -> None:
     if t.dtype != torch.int32 or t.device != device or not t.is_contiguous() or t.dim() != 1:
         raise ValueError(f"{name} must be a contiguous one-dimensional int32 tensor on {device}")
-    if shape is not None and tuple(t.shape) != shape:
+    if shape is not None and t.shape != shape:
         raise ValueError(f"{name} has shape {tuple(t.shape)}, not {shape}")
 
 
