@@ -668,8 +668,8 @@ adapter_gemm_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_consta
 }
 
 // ------------------------------------------------------------------------------------------------------------------------------------
-// fp32: true 32-bit multiply-adds.  The low-rank rows first, a block per token; then the projection in tiles of 64 features x TN tokens, a
-// thread summing 4 x NT of them, whose epilogue adds each token's low-rank term.  Clusters split K where the tiles are few.
+// fp32: true 32-bit multiply-adds.  The low-rank rows first, a block per token; then the projection in tiles of 64 features, whose epilogue adds
+// each token's low-rank term.  Clusters split K where the tiles are few.
 // Sums run over 128 products in one accumulator, which is then added to another: a plain chain over K = 7064 was off by five times as much
 // (1.1e-6 of the outputs' scale against 2e-7).
 // ------------------------------------------------------------------------------------------------------------------------------------
