@@ -304,7 +304,8 @@ constexpr int LOW_RING = 208 * 1024;     // bytes; the sums of a pass (160 KB) t
 
 // Prompts, 128 tokens: the tokens are the MMA's rows and up to 16 panels its columns, those of the adapters that these tokens have, so that a
 // k-block moves the tokens once and the factors of these adapters; the panels of the tile's other adapters get zeros.  Cluster (1, 1, CS)
-// splits K.
+// splits K; where token tiles are few, blocks side by side take 16 panels each (512 tokens of 256 adapters of rank 16, 4096 -> 4096: 223 us a
+// call one after another, 120 so).
 __global__ void __launch_bounds__(TC_THREADS, 1)
 adapter_low_prompt_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmX, const LowArgs a) {
   constexpr int PASS = LOW_PASS, TMEM_COLS = PASS * 16, PITCH = LOW_PITCH;
@@ -319,7 +320,8 @@ adapter_low_prompt_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 1);
   const int warp = uniform_warp(), lane = threadIdx.x & 31;
   const int token0 = blockIdx.y * 128, tile = token0 / PLAN_TILE;
-  const int count = min(a.counts[tile], a.capacity);
+  const int count = min(a.counts[tile], a.capacity), pass = PASS / a.run * a.run, p_first = blockIdx.x * pass;
+  if (p_first > 0 && p_first >= count * a.all_panels) return;   // blocks for more adapters than the tile has
   __shared__ int who[128], slot[PLAN_TILE];
   __shared__ float scale[128];
   __shared__ short place[PLAN_TILE], active[128];   // of the list's adapters: which of the active ones, -1: none; and back
@@ -328,7 +330,7 @@ adapter_low_prompt_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_
 
   const int kb0 = part_begin(a.kb, blockIdx.z, gridDim.z), kb1 = part_begin(a.kb, blockIdx.z + 1, gridDim.z);
   // as many stages as the ring holds for the panels that these tokens may have
-  const int pass = PASS / a.run * a.run, stage = W_BYTES + min(pass, count * a.all_panels) * 2048, stages = min(LOW_STAGES, LOW_RING / stage);
+  const int stage = W_BYTES + min(pass, count * a.all_panels) * 2048, stages = min(LOW_STAGES, LOW_RING / stage);
   const int pre = count > 0 ? min(stages, kb1 - kb0) : 0;   // as above
   if (warp == 0 && elect_one()) {
     for (int s = 0; s < stages; ++s) {
@@ -368,13 +370,13 @@ adapter_low_prompt_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_
   }
   __syncthreads();
   const int panels = n_active * a.all_panels;
-  if (panels == 0 && warp == 0 && elect_one()) {   // the tokens loaded ahead are not needed: only let them land
+  if (p_first >= panels && warp == 0 && elect_one()) {   // the tokens loaded ahead are not needed: only let them land
     for (int i = 0; i < pre; ++i) {
       mbar_expect_tx(&full[i], W_BYTES);
       (void)mbar_wait(&full[i], 0, 4);
     }
   }
-  if (warp >= 2) {   // zeros for adapters that only the tile's other 128 tokens have
+  if (blockIdx.x == 0 && warp >= 2) {   // zeros for adapters that only the tile's other 128 tokens have
     const int cs = gridDim.z, share = 128 / cs;
     bf16* const h = a.h + (size_t)tile * a.capacity * a.all_panels * a.tile_rows * 16;
     for (int j = 0; j < count; ++j)
@@ -387,7 +389,7 @@ adapter_low_prompt_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_
   int s = 0, round = 0;
   uint32_t parity = 0;
   bool ok = true;
-  for (int p0 = 0; p0 < panels; p0 += pass, ++round) {
+  for (int p0 = p_first; p0 < panels; p0 += gridDim.x * pass, ++round) {
     const int np = min(pass, panels - p0);
     if (warp == 0) {
       if (elect_one() && ok) {
@@ -1021,7 +1023,9 @@ int launch_low_prompt(const Call& c) {
   int rc = prism_get_tensor_map(c.a, (unsigned long long)c.terms.slots * a.all_panels * 16, (unsigned long long)c.K, (unsigned long long)c.K, 16 * a.run, &ta);
   if (!rc) rc = prism_get_tensor_map(c.x, (unsigned long long)c.T, (unsigned long long)c.K, (unsigned long long)c.ldx, 128, &tx);
   if (rc) return rc;
-  return (int)prism_launch_clusters(adapter_low_prompt_kernel, dim3(1, tiles, cs), dim3(TC_THREADS), smem, c.stream, c.pdl, cs, ta, tx, a);
+  const int pass = LOW_PASS / a.run * a.run, passes = (a.capacity * a.all_panels + pass - 1) / pass, places = SMS / (tiles * cs);
+  const int gx = places < 1 ? 1 : places < passes ? places : passes;
+  return (int)prism_launch_clusters(adapter_low_prompt_kernel, dim3(gx, tiles, cs), dim3(TC_THREADS), smem, c.stream, c.pdl, cs, ta, tx, a);
 }
 
 template <int BN, bool DUAL>
@@ -1090,9 +1094,13 @@ int launch_decode(const Call& c) {
 }
 
 int launch_prompt(Call& c) {
-  const bool pair = prism_adapter_pair_fits(c.M, c.act != 0, c.terms, c.out, c.ldo, c.bias);
+  bool pair = prism_adapter_pair_fits(c.M, c.act != 0, c.terms, c.out, c.ldo, c.bias);
   int bn;
   c.pair_tiles = pair ? prism_adapter_pair_tiles(c.M, c.T, c.act != 0, c.terms, &bn) : 0;
+  // A pair of SMs adds all panels of its token tile one after another (0.8 us for four, their copies' issue); the blocks of a decode form's cluster
+  // share them out.  Up to 256 tokens that may have many adapters, where the pairs would have no second tile to hide that behind, run as two decode
+  // tiles: 4096 -> 4096, 256 tokens, 256 / 16 adapters of rank 16: 66 / 28 us, on pairs 115 / 26; 160 tokens, 40 / 4 adapters: 27 / 21 and 43 / 23.
+  if (pair && c.T <= PLAN_TILE && c.pair_tiles <= SMS / 2 && c.terms.capacity * c.terms.panels > 16) pair = false, c.pair_tiles = 0;
   const int rc = launch_low_prompt(c);
   if (rc) return rc;
   if (pair)
