@@ -234,8 +234,8 @@ def _run_f32(x, w, pool, p, bias, out, act):
 
 def linear(x: torch.Tensor, w: torch.Tensor, pool: AdapterPool, p: AdapterPlan, *, bias: Optional[torch.Tensor] = None,
            out: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """``x @ w.T + bias`` and every token's adapter; x ``[T, K]``, w ``[M, K]`` -> ``[T, M]``, sums in 32 bits, rounded once.  ``out``
-    shares no memory with the inputs."""
+    """``x @ w.T + bias`` and every token's adapter; x ``[T, K]``, w ``[M, K]`` -> ``[T, M]``.  Sums and scale in 32 bits; in bf16 the low-rank
+    row is rounded once, as an operand of the matrix instructions, and so is the result.  ``out`` shares no memory with the inputs."""
     _check(x, w, pool, p, bias, out, pool.features)
     if not x.is_cuda:
         y = _adapted_cpu(x, w, pool, p, bias).to(x.dtype)
@@ -248,7 +248,7 @@ def linear(x: torch.Tensor, w: torch.Tensor, pool: AdapterPool, p: AdapterPlan, 
 def gate_up_glu(x: torch.Tensor, w_gate_up: torch.Tensor, pool: AdapterPool, p: AdapterPlan, act: str, *,
                 out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``act(gate) * up`` with ``w_gate_up = [Wg ; Wu]`` and the adapters of both (a pool of two equal sections); ``act`` is ``silu`` or
-    ``gelu_tanh``.  Sums, activation and product in 32 bits, rounded once."""
+    ``gelu_tanh``.  Sums, activation and product in 32 bits, rounded as ``linear`` rounds."""
     if act not in ("silu", "gelu_tanh"):
         raise ValueError(f"act {act!r} is neither silu nor gelu_tanh")
     if len(pool.sections) != 2 or pool.sections[0] != pool.sections[1]:

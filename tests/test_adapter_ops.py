@@ -10,7 +10,7 @@ sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
 from op_helpers import CPU, GPU16, GPU32, rand  # noqa: E402
 
 from prism_infer_b200 import ops  # noqa: E402
-from prism_infer_b200.ops import adapters, native  # noqa: E402
+from prism_infer_b200.ops import adapters, batch, native  # noqa: E402
 
 BACKENDS = [CPU, GPU32, GPU16]
 GPU = [GPU32, GPU16]
@@ -330,6 +330,16 @@ def test_slots_out_of_range_count_as_none_and_are_reported():
     assert native.read_status()["adapters"][0] == 3
     p.plan, p.who[2:5] = plan, -1
     p.check(p.run())
+
+
+@pytest.mark.gpu
+def test_tensors_of_another_device_than_the_current_one_are_refused(monkeypatch):
+    p = Problem(("cuda:0", torch.bfloat16), 4, 64, (32,), 8, 2, [0, 1, -1, 0])
+    lengths = torch.ones(1, dtype=torch.int32, device="cuda:0")
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 1)
+    for call in (p.run, lambda: adapters.plan(p.plan.adapter, 2), lambda: batch.step_maps(lengths, lengths, lengths, page=16, tokens=1, width=1)):
+        with pytest.raises(ValueError):
+            call()
 
 
 @pytest.mark.parametrize("backend", BACKENDS)
