@@ -31,8 +31,9 @@ MAX_RANK = 256
 class AdapterPool:
     """Factors of one projection ``[sum(sections), in_features]`` for up to ``slots`` adapters of rank up to ``rank`` per section, laid
     out as the kernels read them: ``a [slots, sections * panels * 16, in_features]``, ``b [slots, panels, rows, 16]`` with every section's
-    features padded to a multiple of 8 rows (in bf16 the ranks of 8 rows as ``[2, 8 rows, 8 ranks]``), ``scale [slots]``.  A slot that was
-    never loaded adds nothing."""
+    features padded to a multiple of 8 rows (in bf16 the ranks of 8 rows as ``[2, 8 rows, 8 ranks]``), ``scale [slots]``,
+    ``ranks [slots, sections]``.  A slot that was never loaded adds nothing.  What a slot holds beyond its own ranks is padding: it
+    takes no part in the result, but is read and multiplied like the rest."""
 
     def __init__(self, slots: int, rank: int, in_features: int, sections: Union[int, Sequence[int]], *, device,
                  dtype: torch.dtype = torch.bfloat16):
@@ -55,6 +56,7 @@ class AdapterPool:
         self.a = torch.zeros(slots, self.low, in_features, dtype=dtype, device=device)
         self.b = torch.zeros(slots, self.panels, self.rows, PANEL, dtype=dtype, device=device)
         self.scale = torch.zeros(slots, dtype=torch.float32, device=device)
+        self.ranks = torch.zeros(slots, len(sections), dtype=torch.int32, device=device)
         self.device = self.a.device
         ends = [sum(sections[:i + 1]) for i in range(len(sections))]
         self._ends = (ctypes.c_int * len(ends))(*ends)
@@ -86,6 +88,8 @@ class AdapterPool:
         self.a[slot] = pa.view(self.low, self.in_features)
         self.b[slot] = self._panels(pb.view(self.rows, self.panels, PANEL).transpose(0, 1))
         self.scale[slot] = float(scale)
+        for i, fa in enumerate(a):
+            self.ranks[slot, i] = fa.shape[0]
 
     def _panels(self, b: torch.Tensor) -> torch.Tensor:
         """``[panels, rows, 16]`` in the pool's order."""
@@ -107,6 +111,7 @@ class AdapterPool:
         self.a[slot] = 0
         self.b[slot] = 0
         self.scale[slot] = 0
+        self.ranks[slot] = 0
 
 
 @dataclass
@@ -186,7 +191,8 @@ def _adapted_cpu(x, w, pool, p, bias):
         low = F.linear(x[rows].float(), pool.a[s].float()) * pool.scale[s]
         first, r = 0, pool.panels * PANEL
         for i, m in enumerate(pool.sections):
-            y[rows, first:first + m] += F.linear(low[:, i * r:(i + 1) * r], pool._features(s, i).float())
+            n = int(pool.ranks[s, i])
+            y[rows, first:first + m] += F.linear(low[:, i * r:i * r + n], pool._features(s, i)[:, :n].float())
             first += m
     return y
 
@@ -217,7 +223,7 @@ def _run(x, w, pool, p, bias, out, act):
     while T > 0:
         if n > T:       # the last run of several
             n, tile_rows = T, _tile_rows(T)
-        native.call("prism_adapter_linear", x_at, w.data_ptr(), pool.a.data_ptr(), pool.b.data_ptr(), pool.scale.data_ptr(), index_at, lists_at, counts_at,
+        native.call("prism_adapter_linear", x_at, w.data_ptr(), pool.a.data_ptr(), pool.b.data_ptr(), pool.scale.data_ptr(), pool.ranks.data_ptr(), index_at, lists_at, counts_at,
                     _p(bias), out_at, h.data_ptr(), n, *rest, tile_rows, act, ldx, _ld(w), ldo, _s(), _pdl())
         x_at, out_at, index_at = x_at + 2 * n * ldx, out_at + 2 * n * ldo, index_at + 4 * n
         lists_at, counts_at, T = lists_at + 4 * run * capacity, counts_at + 4 * run, T - n
@@ -227,7 +233,7 @@ def _run(x, w, pool, p, bias, out, act):
 def _run_f32(x, w, pool, p, bias, out, act):
     T = x.shape[0]
     h = torch.empty(T, pool.low, dtype=torch.float32, device=x.device)
-    native.call("prism_adapter_linear_f32", _p(x), _p(w), _p(pool.a), _p(pool.b), _p(pool.scale), _p(p.adapter), _p(bias), _p(out), _p(h), T,
+    native.call("prism_adapter_linear_f32", _p(x), _p(w), _p(pool.a), _p(pool.b), _p(pool.scale), _p(pool.ranks), _p(p.adapter), _p(bias), _p(out), _p(h), T,
                 pool.features, pool.in_features, pool.slots, pool.panels, len(pool.sections), pool._ends, act, _ld(x), _ld(w), _ld(out), _s(), _pdl())
     return out
 
@@ -248,7 +254,8 @@ def linear(x: torch.Tensor, w: torch.Tensor, pool: AdapterPool, p: AdapterPlan, 
 def gate_up_glu(x: torch.Tensor, w_gate_up: torch.Tensor, pool: AdapterPool, p: AdapterPlan, act: str, *,
                 out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``act(gate) * up`` with ``w_gate_up = [Wg ; Wu]`` and the adapters of both (a pool of two equal sections); ``act`` is ``silu`` or
-    ``gelu_tanh``.  Sums, activation and product in 32 bits, rounded as ``linear`` rounds."""
+    ``gelu_tanh``.  Sums, activation and product in 32 bits, rounded as ``linear`` rounds.  In bf16 a row whose low-rank values are
+    infinite becomes not a number: the matrix instructions meet a gate's low-rank row with zeros for the up half, and the other way round."""
     if act not in ("silu", "gelu_tanh"):
         raise ValueError(f"act {act!r} is neither silu nor gelu_tanh")
     if len(pool.sections) != 2 or pool.sections[0] != pool.sections[1]:

@@ -113,8 +113,9 @@ struct LowArgs {
   const int* counts;     // [tiles]
   const int* index;      // [T]
   const float* scale;    // [slots]
+  const int* ranks;      // [slots][sections] of every slot's own factors; the rest of its panels is padding
   bf16* h;               // [tiles][capacity][all_panels] panels of tile_rows tokens
-  int T, kb, capacity, all_panels, tile_rows, stages;
+  int T, kb, capacity, panels, all_panels, tile_rows, stages;   // panels: of one section
   int run;               // panels that one copy moves: a divisor of all_panels, since an adapter's rows of A lie together
 };
 
@@ -124,10 +125,17 @@ __device__ __forceinline__ void load_owners(const LowArgs& a, int* who, int* slo
   for (int c = threadIdx.x; c < TOKENS; c += TC_THREADS) who[c] = token0 + c < a.T ? a.index[token0 + c] : -1;
   for (int j = threadIdx.x; j < min(a.capacity, MOST); j += TC_THREADS) slot[j] = a.lists[(size_t)tile * a.capacity + j];
 }
-// And the scale of every token's adapter; by the epilogue warps, while the sums are under way.
+// And the scale and ranks of every token's adapter; by the epilogue warps, while the sums are under way.
 template <int TOKENS>
-__device__ __forceinline__ void load_scales(const LowArgs& a, const int* who, const int* slot, float* scale) {
-  for (int c = threadIdx.x - 64; c < TOKENS; c += TC_THREADS - 64) scale[c] = who[c] >= 0 ? a.scale[slot[who[c]]] : 0.0f;
+__device__ __forceinline__ void load_scales(const LowArgs& a, const int* who, const int* slot, float* scale, short (*ranks)[MAX_SECTIONS]) {
+  const int sections = a.all_panels / a.panels;
+  for (int c = threadIdx.x - 64; c < TOKENS; c += TC_THREADS - 64) {
+    const int s = who[c] >= 0 ? slot[who[c]] : -1;
+    scale[c] = s >= 0 ? a.scale[s] : 0.0f;
+#pragma unroll
+    for (int k = 0; k < MAX_SECTIONS; ++k)
+      if (k < sections) ranks[c][k] = s >= 0 ? (short)a.ranks[s * sections + k] : 0;
+  }
 }
 
 // Sum over the cluster of four floats that every CTA keeps at the same place.
@@ -151,20 +159,27 @@ __device__ __forceinline__ float4 cluster_sum4(const float* mine, int cs) {
 __device__ __forceinline__ size_t in_panel(int row, int half) { return (size_t)(row >> 3) * 128 + half * 64 + (row & 7) * 8; }
 
 // Panels of h from the sums in `red`, of which every CTA of the cluster holds a part: each CTA adds up and stores its share of the tokens,
-// zeros in panels of adapters that are not the token's.  panel_at(g) is the g-th of the np panels.
+// zeros in panels of adapters that are not the token's and in the padding of its own: a row with an infinite value has sums there that are no
+// numbers, and these would stay so through the padding's zeros in B.  panel_at(g) is the g-th of the np panels.
 template <int PITCH, bool TOKEN_MAJOR, int TOKENS, typename PanelAt>
-__device__ __forceinline__ void store_low_rows(const LowArgs& a, const float* red, const int* who, const float* scale, PanelAt panel_at, int np, int token0,
-                                               int tile) {
+__device__ __forceinline__ void store_low_rows(const LowArgs& a, const float* red, const int* who, const float* scale, const short (*ranks)[MAX_SECTIONS],
+                                               PanelAt panel_at, int np, int token0, int tile) {
   const int cs = gridDim.z, share = TOKENS / cs, first = blockIdx.z * share, shift = __ffs(share) - 1;   // a power of two
   bf16* const h = a.h + (size_t)tile * a.capacity * a.all_panels * a.tile_rows * 16;
   for (int i = threadIdx.x; i < np * share * 2; i += TC_THREADS) {   // items of eight ranks
     const int half = (i >> shift) & 1, c = first + (i & (share - 1)), g = i >> (1 + shift), p = panel_at(g), own = p - who[c] * a.all_panels;
     uint4 o = make_uint4(0, 0, 0, 0);
+    int left = 0;   // of these eight ranks, the adapter has so many
     if (who[c] >= 0 && own >= 0 && own < a.all_panels) {
+      const int section = own / a.panels;
+      left = ranks[c][section] - (own - section * a.panels) * 16 - half * 8;
+    }
+    if (left > 0) {
       const float* const mine = red + (TOKEN_MAJOR ? c * PITCH + g * 16 : (g * TOKENS + c) * PITCH) + half * 8;
       const float4 v = cluster_sum4(mine, cs), u = cluster_sum4(mine + 4, cs);
       const float f = scale[c];
-      const uint2 lo = pack4(make_float4(v.x * f, v.y * f, v.z * f, v.w * f)), hi = pack4(make_float4(u.x * f, u.y * f, u.z * f, u.w * f));
+      const uint2 lo = pack4(make_float4(v.x * f, left > 1 ? v.y * f : 0.0f, left > 2 ? v.z * f : 0.0f, left > 3 ? v.w * f : 0.0f));
+      const uint2 hi = pack4(make_float4(left > 4 ? u.x * f : 0.0f, left > 5 ? u.y * f : 0.0f, left > 6 ? u.z * f : 0.0f, left > 7 ? u.w * f : 0.0f));
       o = make_uint4(lo.x, lo.y, hi.x, hi.y);
     }
     *reinterpret_cast<uint4*>(h + (size_t)p * a.tile_rows * 16 + in_panel(token0 - tile * PLAN_TILE + c, half)) = o;
@@ -194,6 +209,7 @@ adapter_low_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
   const int panels = min(a.counts[0], min(a.capacity, BN)) * a.all_panels;
   __shared__ int who[BN], slot[BN];   // no more adapters than tokens
   __shared__ float scale[BN];
+  __shared__ short ranks[BN][MAX_SECTIONS];
 
   const int kb0 = part_begin(a.kb, blockIdx.z, gridDim.z), kb1 = part_begin(a.kb, blockIdx.z + 1, gridDim.z);
   // the first tokens are under way before the list of adapters is read; their bytes are announced with those of the factors
@@ -273,7 +289,7 @@ adapter_low_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
         if (ok) tc_commit(acc_full);
       }
     } else {
-      if (round == 0) load_scales<BN>(a, who, slot, scale);
+      if (round == 0) load_scales<BN>(a, who, slot, scale, ranks);
       // rows of unused panels hold what earlier loads left; nothing reads them
       ok = ok && __all_sync(0xffffffffu, mbar_wait(acc_full, round & 1, 3));
       if (ok) {
@@ -285,7 +301,7 @@ adapter_low_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
     __syncwarp();
     cluster_sync_all();
     tc_fence_after();
-    store_low_rows<PITCH, true, BN>(a, red, who, scale, [&](int g) { return p0 + g; }, np, 0, 0);
+    store_low_rows<PITCH, true, BN>(a, red, who, scale, ranks, [&](int g) { return p0 + g; }, np, 0, 0);
     // the ring is written again by copies once every CTA has read the sums
     fence_proxy_async();
     cluster_sync_all();
@@ -324,6 +340,7 @@ adapter_low_prompt_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_
   if (p_first > 0 && p_first >= count * a.all_panels) return;   // blocks for more adapters than the tile has
   __shared__ int who[128], slot[PLAN_TILE];
   __shared__ float scale[128];
+  __shared__ short ranks[128][MAX_SECTIONS];
   __shared__ short place[PLAN_TILE], active[128];   // of the list's adapters: which of the active ones, -1: none; and back
   __shared__ int n_active;
   for (int j = threadIdx.x; j < count; j += TC_THREADS) place[j] = -1;
@@ -434,7 +451,7 @@ adapter_low_prompt_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_
         if (ok) tc_commit(acc_full);
       }
     } else {
-      if (round == 0) load_scales<128>(a, who, slot, scale);
+      if (round == 0) load_scales<128>(a, who, slot, scale, ranks);
       const int q = warp & 3, c = q * 32 + lane, first_own = who[c] < 0 ? panels : place[who[c]] * a.all_panels;
       ok = ok && __all_sync(0xffffffffu, mbar_wait(acc_full, round & 1, 3));
       if (ok) {
@@ -461,7 +478,7 @@ adapter_low_prompt_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_
       const int k = (p0 + g) / a.all_panels;
       return active[k] * a.all_panels + (p0 + g - k * a.all_panels);
     };
-    store_low_rows<PITCH, false, 128>(a, red, who, scale, panel_at, np, token0, tile);
+    store_low_rows<PITCH, false, 128>(a, red, who, scale, ranks, panel_at, np, token0, tile);
     fence_proxy_async();
     cluster_sync_all();
   }
@@ -679,9 +696,10 @@ struct LowF32Args {
   const float* x;       // [T][ldx]
   const float* a;       // [slots][low][K]
   const float* scale;   // [slots]
+  const int* ranks;     // [slots][sections]
   const int* adapter;   // [T]
   float* h;             // [T][low]; rows of tokens without an adapter are not written
-  int K, low, slots;
+  int K, low, slots, padded;   // padded: ranks of a section
   long long ldx;
 };
 
@@ -723,7 +741,9 @@ __global__ void __launch_bounds__(256) adapter_low_f32_kernel(const LowF32Args a
       }
     }
     const float u = warp_sum((s0.x + s0.y) + (s0.z + s0.w)), w = warp_sum((s1.x + s1.y) + (s1.z + s1.w));
-    if (lane < 2) a.h[(size_t)t * a.low + r + lane] = (lane ? w : u) * scale;
+    // zeros in the padding, as in bf16; both rows are of one section
+    const int section = r / a.padded, rank = a.ranks[who * (a.low / a.padded) + section];
+    if (lane < 2) a.h[(size_t)t * a.low + r + lane] = r + lane - section * a.padded < rank ? (lane ? w : u) * scale : 0.0f;
   }
 }
 
@@ -892,13 +912,13 @@ constexpr int SMEM_LIMIT = 232448 - 4096;   // 227 KB, 4 KB of it for static arr
 
 // Dynamic shared memory above 48 KB has to be allowed once per kernel and device.
 template <typename Kernel>
-cudaError_t allow_smem(Kernel kernel, std::atomic<unsigned long long>& devices) {
+cudaError_t allow_smem(Kernel kernel, std::atomic<unsigned long long>& devices, int bytes = SMEM_LIMIT) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   const unsigned long long bit = 1ull << (dev & 63);
   if (devices.load(std::memory_order_acquire) & bit) return cudaSuccess;
-  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_LIMIT);
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
   if (e == cudaSuccess) devices.fetch_or(bit, std::memory_order_release);
   return e;
 }
@@ -919,6 +939,7 @@ struct Call {
   long long ldx, ldw;
   const void *a, *b;
   const float* scale;
+  const int* ranks;
   const int* index;
   PrismAdapterTerms terms;
   const void* bias;
@@ -981,8 +1002,8 @@ int panel_run(int all_panels, int pass, int unused) {
 }
 
 LowArgs low_args(const Call& c, int pass, int unused) {
-  return LowArgs{c.terms.lists, c.terms.counts, c.index, c.scale, (bf16*)c.h, c.T, (c.K + 63) / 64, c.terms.capacity, c.terms.panels * c.terms.sec.n,
-                 c.tile_rows, 0, panel_run(c.terms.panels * c.terms.sec.n, pass, unused)};
+  return LowArgs{c.terms.lists, c.terms.counts, c.index, c.scale, c.ranks, (bf16*)c.h, c.T, (c.K + 63) / 64, c.terms.capacity, c.terms.panels,
+                 c.terms.panels * c.terms.sec.n, c.tile_rows, 0, panel_run(c.terms.panels * c.terms.sec.n, pass, unused)};
 }
 
 template <int BN, int G>
@@ -1007,12 +1028,12 @@ int launch_low(const Call& c) {
 int launch_low_prompt(const Call& c) {
   static std::atomic<unsigned long long> devices{0};
   static ClusterTable table;
-  cudaError_t e = allow_smem(adapter_low_prompt_kernel, devices);
+  const size_t smem = 1024 + LOW_RING + (2 * LOW_STAGES + 1) * 8 + 16;
+  cudaError_t e = allow_smem(adapter_low_prompt_kernel, devices, (int)smem);
   if (e != cudaSuccess) return (int)e;
   LowArgs a = low_args(c, LOW_PASS, LOW_PASS / 4);
   const int tiles = (c.T + 127) / 128;
   static_assert(LOW_PASS * 128 * LOW_PITCH * 4 <= LOW_RING, "the sums fit the ring");
-  const size_t smem = 1024 + LOW_RING + (2 * LOW_STAGES + 1) * 8 + 16;
   // The projection's pairs of SMs that walk one tile more than the others are its first blocks.  Where there are SMs for them beside these
   // blocks they start at once, and the others have as much time for the low-rank rows as a tile takes (8192 tokens, 4096 -> 6144 qkv: 64
   // blocks, 300 us; 128 blocks, whose rows take half the time, 306).  Where most pairs walk one tile more the rows come first, as fast as may be.
@@ -1154,14 +1175,14 @@ int launch_f32(const TileF32Args& a, bool vec, cudaStream_t on) {
 }  // namespace
 
 // The same in 32 bits; b: [slots][panels][rows][16], h: T x low floats of workspace.
-PRISM_API int prism_adapter_linear_f32(const void* x, const void* w, const void* a, const void* b, const void* scale, const void* adapter,
+PRISM_API int prism_adapter_linear_f32(const void* x, const void* w, const void* a, const void* b, const void* scale, const void* ranks, const void* adapter,
                                        const void* bias, void* out, void* h, int T, int M, int K, int slots, int panels, int sections, const void* ends,
                                        int act, long long ldx, long long ldw, long long ldo, void* stream, int pdl) {
   if (T < 1 || T > 65535 * 64 || M < 1 || K < 1 || slots < 1 || panels < 1 || sections < 1 || sections > MAX_SECTIONS) return -1;
   if (act && (M % 2 || sections != 2 || bias != nullptr)) return -2;
   const bool vec = (((uintptr_t)x | (uintptr_t)w | (uintptr_t)a) & 15) == 0 && K % 4 == 0 && ldx % 4 == 0 && ldw % 4 == 0;
   const int low = sections * panels * 16;
-  LowF32Args l{(const float*)x, (const float*)a, (const float*)scale, (const int*)adapter, (float*)h, K, low, slots, ldx};
+  LowF32Args l{(const float*)x, (const float*)a, (const float*)scale, (const int*)ranks, (const int*)adapter, (float*)h, K, low, slots, panels * 16, ldx};
   // few tokens: a block per 16 rows
   const cudaError_t e = prism_launch(vec ? adapter_low_f32_kernel<true> : adapter_low_f32_kernel<false>, dim3(T, T < 148 ? (low + 15) / 16 : 1), dim3(256), 0, (cudaStream_t)stream, pdl != 0, l);
   if (e != cudaSuccess) return (int)e;
@@ -1180,8 +1201,8 @@ PRISM_API int prism_adapter_linear_f32(const void* x, const void* w, const void*
 }
 
 // bf16 projection (act 0) or gated unit (PRISM_GLU_*) with the adapters of a plan.  lists, counts: of the call's tiles of 256 tokens;
-// b: [slots][panels] panels; h: tiles x capacity x all panels x tile_rows x 16 bf16 of workspace, tile_rows 16, 32, 64, 128 (as many as the tokens need) or 256.
-PRISM_API int prism_adapter_linear(const void* x, const void* w, const void* a, const void* b, const void* scale, const void* index,
+// b: [slots][panels] panels; ranks: [slots][sections]; h: tiles x capacity x all panels x tile_rows x 16 bf16 of workspace, tile_rows 16, 32, 64, 128 (as many as the tokens need) or 256.
+PRISM_API int prism_adapter_linear(const void* x, const void* w, const void* a, const void* b, const void* scale, const void* ranks, const void* index,
                                    const void* lists, const void* counts, const void* bias, void* out, void* h, int T, int M, int K, int slots,
                                    int panels, int sections, const void* ends, int capacity, int tile_rows, int act, long long ldx, long long ldw,
                                    long long ldo, void* stream, int pdl) {
@@ -1197,6 +1218,7 @@ PRISM_API int prism_adapter_linear(const void* x, const void* w, const void* a, 
   c.a = a;
   c.b = b;
   c.scale = (const float*)scale;
+  c.ranks = (const int*)ranks;
   c.index = (const int*)index;
   c.terms.h = h;
   c.terms.b = b;

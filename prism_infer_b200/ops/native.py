@@ -79,8 +79,8 @@ _SIGNATURES = {
     "prism_kv_compact": "pliplppppiiiip",
     "prism_step_maps": "pppppp" "iiiii" "ppppppppp" "pi",
     "prism_adapter_plan": "piiippppi",
-    "prism_adapter_linear_f32": "ppppppppp" "iiiiii" "pilllpi",
-    "prism_adapter_linear": "ppppp" "pppp" "pp" "iiiiii" "piii" "lllpi",
+    "prism_adapter_linear_f32": "pppppppppp" "iiiiii" "pilllpi",
+    "prism_adapter_linear": "pppppp" "pppp" "pp" "iiiiii" "piii" "lllpi",
     "prism_sample": "pllipppiilupppipi",
     "prism_merge_candidates": "pppiipi",
     "prism_lm_head_fp8_plan": "p",

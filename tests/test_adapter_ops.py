@@ -387,3 +387,44 @@ def test_refusals(backend):
     refused(pool.clear, -1)
     if device == "cpu":
         refused(adapters.plan, torch.tensor([2], dtype=torch.int32), 2)
+
+
+@pytest.mark.parametrize("backend", BACKENDS)
+@pytest.mark.parametrize("T", [3, 40, 200, 300])
+def test_infinite_rows_meet_the_ranks_of_their_own_adapter_only(backend, T):
+    """Slots are padded to the pool's rank.  Padding times infinity is no number, and takes no part: a row with an infinite value gets what
+    its adapter's own ranks make of it, and an empty slot adds nothing to it."""
+    ranks = [(20, 20), (3, 17), (16, 1)]                 # of three slots, by section; the fourth stays empty
+    p = Problem(backend, T, 64, (40, 24), 20, 4, torch.arange(T, dtype=torch.int32) % 5 - 1)
+    p.pool.clear(3)
+    p.a, p.w = p.a.abs() + 2.0 ** -6, p.w.abs() + 2.0 ** -6
+    p.b = [b.abs() + 2.0 ** -6 for b in p.b]
+    p.a, p.w, p.b = p.a.bfloat16().float(), p.w.bfloat16().float(), [b.bfloat16().float() for b in p.b]
+    for s in range(4):
+        for i in range(2):
+            own = ranks[s][i] if s < 3 else 0
+            p.a[s, i, own:], p.b[i][s, :, own:] = 0, 0
+        if s < 3:
+            p.pool.load(s, [p.a[s, i, :r] for i, r in enumerate(ranks[s])], [p.b[i][s, :, :r] for i, r in enumerate(ranks[s])], p.scale[s])
+    bad = torch.arange(T) % 7 < 5 if T > 3 else torch.tensor([True, False, True])
+    clean = p.run().clone()
+    p.check(clean)
+    p.x[bad, 9] = float("inf")                           # every weight and factor that it meets is positive
+    got = p.run()
+    assert torch.equal(got[~bad.to(got.device)], clean[~bad.to(got.device)])
+    assert bool((got[bad.to(got.device)] == float("inf")).all())
+
+
+@pytest.mark.parametrize("backend", BACKENDS)
+@pytest.mark.parametrize("T", [3, 200, 300])
+def test_infinite_rows_of_empty_slots_in_a_gated_unit(backend, T):
+    p = Problem(backend, T, 64, (32, 32), 8, 2, torch.arange(T, dtype=torch.int32) % 3 - 1)
+    p.pool.clear(1)
+    p.x[::2, 5] = float("inf")
+    p.x[1::4, 6] = float("nan")
+    got = adapters.gate_up_glu(p.to(p.x), p.to(p.w), p.pool, p.plan, "silu")
+    none = adapters.plan(torch.full((T,), -1, dtype=torch.int32, device=p.device), 2)
+    want = adapters.gate_up_glu(p.to(p.x), p.to(p.w), p.pool, none, "silu")
+    empty = (p.who != 0).to(got.device)
+    assert torch.equal(got[empty].isnan(), want[empty].isnan())
+    assert torch.equal(got[empty].nan_to_num(nan=0.5), want[empty].nan_to_num(nan=0.5))
