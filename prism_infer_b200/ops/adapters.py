@@ -197,8 +197,10 @@ def _adapted_cpu(x, w, pool, p, bias):
     return y
 
 
-# bytes of low-rank rows in one launch; a step that needs more runs in runs of tokens
+# bytes of bf16 low-rank rows in one launch, and tokens of either type (tiles of 128 along an axis of the grid); a step that needs more runs in
+# runs of tokens
 MAX_LOW_BYTES = 256 << 20
+MAX_RUN = 65535 * 128
 
 
 def _tile_rows(tokens: int) -> int:
@@ -215,7 +217,7 @@ def _run(x, w, pool, p, bias, out, act):
     tiles, capacity = p.lists.shape
     tile_rows, ldx, ldo = _tile_rows(T), _ld(x), _ld(out)
     per_tile = capacity * pool.low * tile_rows     # values of every panel that a tile's adapters may need
-    run = min(tiles, max(1, MAX_LOW_BYTES // (2 * per_tile)))
+    run = min(tiles, max(1, MAX_LOW_BYTES // (2 * per_tile)), MAX_RUN // TILE_TOKENS)
     h = torch.empty(run * per_tile, dtype=torch.bfloat16, device=x.device)
     x_at, out_at, index_at, lists_at, counts_at = x.data_ptr(), out.data_ptr(), p.index.data_ptr(), p.lists.data_ptr(), p.counts.data_ptr()
     rest = (pool.features, pool.in_features, pool.slots, pool.panels, len(pool.sections), pool._ends, capacity)
@@ -231,10 +233,12 @@ def _run(x, w, pool, p, bias, out, act):
 
 
 def _run_f32(x, w, pool, p, bias, out, act):
-    T = x.shape[0]
-    h = torch.empty(T, pool.low, dtype=torch.float32, device=x.device)
-    native.call("prism_adapter_linear_f32", _p(x), _p(w), _p(pool.a), _p(pool.b), _p(pool.scale), _p(pool.ranks), _p(p.adapter), _p(bias), _p(out), _p(h), T,
-                pool.features, pool.in_features, pool.slots, pool.panels, len(pool.sections), pool._ends, act, _ld(x), _ld(w), _ld(out), _s(), _pdl())
+    T, ldx, ldo = x.shape[0], _ld(x), _ld(out)
+    h = torch.empty(min(T, MAX_RUN), pool.low, dtype=torch.float32, device=x.device)
+    for first in range(0, T, MAX_RUN):
+        native.call("prism_adapter_linear_f32", x.data_ptr() + 4 * first * ldx, _p(w), _p(pool.a), _p(pool.b), _p(pool.scale), _p(pool.ranks),
+                    p.adapter.data_ptr() + 4 * first, _p(bias), out.data_ptr() + 4 * first * ldo, _p(h), min(MAX_RUN, T - first), pool.features,
+                    pool.in_features, pool.slots, pool.panels, len(pool.sections), pool._ends, act, ldx, _ld(w), ldo, _s(), _pdl())
     return out
 
 

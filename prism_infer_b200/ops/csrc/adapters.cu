@@ -18,6 +18,7 @@ typedef __nv_bfloat16 bf16;
 constexpr int PLAN_TILE = 256;          // tokens that share a list of adapters
 constexpr int PLAN_MAX_SLOTS = 8192;
 constexpr int MAX_SECTIONS = 8;
+constexpr int MAX_TOKENS = 65535 * 128; // of a call: tiles of 128 along one axis of the grid
 
 enum { ADAPTER_SLOT = 1 };              // detail of a failed bounds check
 
@@ -1178,7 +1179,7 @@ int launch_f32(const TileF32Args& a, bool vec, cudaStream_t on) {
 PRISM_API int prism_adapter_linear_f32(const void* x, const void* w, const void* a, const void* b, const void* scale, const void* ranks, const void* adapter,
                                        const void* bias, void* out, void* h, int T, int M, int K, int slots, int panels, int sections, const void* ends,
                                        int act, long long ldx, long long ldw, long long ldo, void* stream, int pdl) {
-  if (T < 1 || T > 65535 * 64 || M < 1 || K < 1 || slots < 1 || panels < 1 || sections < 1 || sections > MAX_SECTIONS) return -1;
+  if (T < 1 || T > MAX_TOKENS || M < 1 || K < 1 || slots < 1 || panels < 1 || sections < 1 || sections > MAX_SECTIONS) return -1;
   if (act && (M % 2 || sections != 2 || bias != nullptr)) return -2;
   const bool vec = (((uintptr_t)x | (uintptr_t)w | (uintptr_t)a) & 15) == 0 && K % 4 == 0 && ldx % 4 == 0 && ldw % 4 == 0;
   const int low = sections * panels * 16;
@@ -1206,7 +1207,7 @@ PRISM_API int prism_adapter_linear(const void* x, const void* w, const void* a, 
                                    const void* lists, const void* counts, const void* bias, void* out, void* h, int T, int M, int K, int slots,
                                    int panels, int sections, const void* ends, int capacity, int tile_rows, int act, long long ldx, long long ldw,
                                    long long ldo, void* stream, int pdl) {
-  if (T < 1 || M < 1 || K < 1 || K % 8 || slots < 1 || panels < 1 || sections < 1 || sections > MAX_SECTIONS || capacity < 1 || capacity > PLAN_TILE) return -1;
+  if (T < 1 || T > MAX_TOKENS || M < 1 || K < 1 || K % 8 || slots < 1 || panels < 1 || sections < 1 || sections > MAX_SECTIONS || capacity < 1 || capacity > PLAN_TILE) return -1;
   if (act && (M % 2 || sections != 2 || bias != nullptr)) return -2;
   const int bn = T <= 16 ? 16 : T <= 32 ? 32 : T <= 64 ? 64 : 128;
   if (tile_rows != (T <= 128 ? bn : PLAN_TILE)) return -3;

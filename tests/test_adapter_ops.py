@@ -428,3 +428,23 @@ def test_infinite_rows_of_empty_slots_in_a_gated_unit(backend, T):
     empty = (p.who != 0).to(got.device)
     assert torch.equal(got[empty].isnan(), want[empty].isnan())
     assert torch.equal(got[empty].nan_to_num(nan=0.5), want[empty].nan_to_num(nan=0.5))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,features", [(torch.bfloat16, 1), (torch.bfloat16, 16), (torch.float32, 1)])
+def test_more_tokens_than_a_grid_has_rows_of_tiles(dtype, features):
+    """65535 blocks of 128 tokens and one token more.  Whole numbers small enough that every sum and product is exact."""
+    T = 65535 * 128 + 1
+    g = torch.Generator("cuda").manual_seed(5)
+
+    def whole(*shape, most):
+        return torch.randint(-most, most + 1, shape, generator=g, device="cuda", dtype=torch.int8).to(dtype)
+
+    x, w, a, b = whole(T, 8, most=2), whole(features, 8, most=2), whole(3, 8, most=1), whole(features, 3, most=1)
+    pool = adapters.AdapterPool(1, 3, 8, features, device="cuda", dtype=dtype)
+    pool.load(0, a, b)
+    who = torch.randint(-1, 1, (T,), generator=g, device="cuda", dtype=torch.int32)
+    got = adapters.linear(x, w, pool, adapters.plan(who, 1))
+    low = x.float() @ a.float().T * (who >= 0)[:, None]
+    assert torch.equal(got.float(), x.float() @ w.float().T + low @ b.float().T)
+    native.check_status()
