@@ -177,7 +177,7 @@ def _check(x: torch.Tensor, w: torch.Tensor, pool: AdapterPool, p: AdapterPlan, 
         raise ValueError(f"out must be {dtype} on {device} of shape {(x.shape[0], features)}, with contiguous rows that are apart")
     for name, t in (("x", x), ("w", w)):
         ld = _ld(t)
-        if t.stride(1) != 1 or ld < K or (dtype == torch.bfloat16 and (ld % 8 or t.data_ptr() % 16)):
+        if (K > 1 and t.stride(1) != 1) or ld < K or (dtype == torch.bfloat16 and (ld % 8 or t.data_ptr() % 16)):
             raise ValueError(f"{name}: rows must be contiguous and apart, in bf16 on 16-byte boundaries")
     check_device(x)
 

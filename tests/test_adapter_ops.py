@@ -448,3 +448,12 @@ def test_more_tokens_than_a_grid_has_rows_of_tiles(dtype, features):
     low = x.float() @ a.float().T * (who >= 0)[:, None]
     assert torch.equal(got.float(), x.float() @ w.float().T + low @ b.float().T)
     native.check_status()
+
+
+@pytest.mark.parametrize("backend", [CPU, GPU32])
+def test_a_single_input_feature_has_any_stride(backend):
+    """Strides of an axis of one element mean nothing."""
+    p = Problem(backend, 5, 1, (6,), 2, 2, [0, 1, -1, 0, 1])
+    x, w = p.to(p.x).reshape(1, 5).t(), p.to(p.w).reshape(1, 6).t()
+    assert x.stride() == (1, 5) and x.is_contiguous() and w.stride() == (1, 6)
+    p.check(adapters.linear(x, w, p.pool, p.plan))
