@@ -457,3 +457,64 @@ def test_a_single_input_feature_has_any_stride(backend):
     x, w = p.to(p.x).reshape(1, 5).t(), p.to(p.w).reshape(1, 6).t()
     assert x.stride() == (1, 5) and x.is_contiguous() and w.stride() == (1, 6)
     p.check(adapters.linear(x, w, p.pool, p.plan))
+
+
+@pytest.mark.parametrize("backend", [CPU, GPU32])
+@pytest.mark.parametrize("T,K,half,rank,slots", [(1, 64, 64, 16, 2), (7, 200, 40, 5, 3), (128, 136, 96, 16, 128), (300, 512, 256, 16, 5), (33, 72, 13, 4, 2)])
+def test_gelu_of_a_gated_unit_in_32_bits(backend, T, K, half, rank, slots):
+    """tanhf, not its approximation: 2^-20 of the unit's scale is sixteen roundings, the approximation is off by 2^-11."""
+    p = Problem(backend, T, K, (half, half), rank, slots, mixed(T, slots))
+    got = adapters.gate_up_glu(p.to(p.x), p.to(p.w), p.pool, p.plan, "gelu_tanh")
+    y, err = p.exact()
+    g, u, eg, eu = y[:, :half], y[:, half:], err[:, :half], err[:, half:]
+    unit = torch.nn.functional.gelu(g, approximate="tanh")
+    p.check(got, unit * u, 1.13 * eg * (u.abs() + eu) + (unit.abs() + 1.13 * eg) * eu + 2.0 ** -20 * (g.abs() + eg) * (u.abs() + eu))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("gated", [False, True])
+def test_pieces_of_two_tiles_have_the_bits_of_one_launch(gated, monkeypatch):
+    """Runs of two tiles of 256 tokens and a shorter one, all of them prompts on pairs of SMs, against the call in one piece; tokens and
+    outputs are columns of wider buffers."""
+    T, sections = 1200, (128, 128)
+    p = Problem(("cuda:0", torch.bfloat16), T, 128, sections, 16, 8, mixed(T, 8), bias=not gated)
+    x = torch.full((T, 160), 7.0, dtype=p.dtype, device=p.device)
+    x[:, 16:144] = p.to(p.x)
+    M = 128 if gated else 256
+
+    def call():
+        out = torch.full((T, M + 32), 3.0, dtype=p.dtype, device=p.device)
+        if gated:
+            adapters.gate_up_glu(x[:, 16:144], p.to(p.w), p.pool, p.plan, "silu", out=out[:, 16:16 + M])
+        else:
+            adapters.linear(x[:, 16:144], p.to(p.w), p.pool, p.plan, bias=p.to(p.bias), out=out[:, 16:16 + M])
+        assert bool((out[:, :16] == 3.0).all()) and bool((out[:, 16 + M:] == 3.0).all())
+        return out[:, 16:16 + M]
+
+    want, calls, launch = call(), [], native.call
+    if not gated:
+        p.check(want)
+    per_tile = 2 * p.plan.lists.shape[1] * p.pool.low * adapters.TILE_TOKENS
+    monkeypatch.setattr(adapters, "MAX_LOW_BYTES", 2 * per_tile + 5)
+    monkeypatch.setattr(native, "call", lambda name, *args: (calls.append(name), launch(name, *args))[1])
+    assert torch.equal(call(), want)
+    assert calls == ["prism_adapter_linear"] * 3
+
+
+@pytest.mark.parametrize("backend", GPU)
+@pytest.mark.parametrize("T", [6, 150, 256, 300])
+def test_rows_of_a_gated_unit_do_not_meet(backend, T):
+    """A row that is infinite or not a number leaves the other rows as they are: decode tiles, two of them, pairs of SMs."""
+    p = Problem(backend, T, 128, (64, 64), 16, 24, mixed(T, 24, bare=0.3))
+
+    def run():
+        return adapters.gate_up_glu(p.to(p.x), p.to(p.w), p.pool, p.plan, "gelu_tanh"), p.run()
+
+    clean = run()
+    bad = torch.tensor([1, T // 2, T - 1])
+    p.x[1, 3], p.x[T // 2], p.x[T - 1, 7] = float("inf"), float("nan"), float("-inf")
+    keep = torch.ones(T, dtype=torch.bool)
+    keep[bad] = False
+    for got, want in zip(run(), clean):
+        assert torch.equal(got[keep.to(got.device)], want[keep.to(got.device)])
+    assert bool(got[T // 2].isnan().all())
