@@ -64,7 +64,7 @@ class AdapterPool:
     @torch.no_grad()
     def load(self, slot: int, a, b, scale: float = 1.0) -> None:
         """``a``: ``[r, in_features]`` and ``b``: ``[features, r]``, or one of each per section; ranks up to the pool's.  The copies are
-        made on the current stream.  Factors that are not finite are refused: tokens of other adapters meet them as products with
+        made on the current stream, and the host waits for them: not for the middle of a step, nor for a captured graph.  Factors that are not finite are refused: tokens of other adapters meet them as products with
         zero."""
         a, b = ([f] if isinstance(f, torch.Tensor) else list(f) for f in (a, b))
         if not 0 <= slot < self.slots:

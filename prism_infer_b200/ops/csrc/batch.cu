@@ -7,9 +7,9 @@
 // pages[start_i + p / page] * page + p % page.
 //
 // A few KB to a few MB move, so a launch is what the step costs: one launch, in which every block adds up all lengths itself (1024
-// requests: 8 KB from L2, one pass over them and one exchange between warps) instead of waiting for a block that does, then writes its
-// share of the tables, 128 entries of a row per warp, and of the tokens, which find their request by halving the running sum in shared
-// memory.  1 request 3.5 us, 1024 requests of up to 8192 tokens in pages of 16 (4 MB, 0.6 us of copy bandwidth) 9.2 us.
+// requests: 8 KB from L2, read twice, for the sums of each thread's requests and, after one exchange between warps, for the sum behind each of
+// them) instead of waiting for a block that does, then writes its share of the tables, 128 entries of a row per warp, and of the tokens, which
+// find their request by halving the running sum in shared memory.  1 request 3.5 us, 1024 requests of up to 8192 tokens in pages of 16 (4 MB, 0.6 us of copy bandwidth) 9.2 us.
 #include "common.cuh"
 
 PRISM_DEFINE_TU_STATUS(batch)
