@@ -64,8 +64,8 @@ class AdapterPool:
     @torch.no_grad()
     def load(self, slot: int, a, b, scale: float = 1.0) -> None:
         """``a``: ``[r, in_features]`` and ``b``: ``[features, r]``, or one of each per section; ranks up to the pool's.  The copies are
-        made on the current stream, and the host waits for them: not for the middle of a step, nor for a captured graph.  Factors that are not finite are refused: tokens of other adapters meet them as products with
-        zero."""
+        made on the current stream, and the host waits for them: not for the middle of a step, nor for a captured graph.  Factors that
+        are not finite are refused: tokens of other adapters meet them as products with zero."""
         a, b = ([f] if isinstance(f, torch.Tensor) else list(f) for f in (a, b))
         if not 0 <= slot < self.slots:
             raise ValueError(f"slot {slot} of {self.slots}")
@@ -225,8 +225,8 @@ def _run(x, w, pool, p, bias, out, act):
     while T > 0:
         if n > T:       # the last run of several
             n, tile_rows = T, _tile_rows(T)
-        native.call("prism_adapter_linear", x_at, w.data_ptr(), pool.a.data_ptr(), pool.b.data_ptr(), pool.scale.data_ptr(), pool.ranks.data_ptr(), index_at, lists_at, counts_at,
-                    _p(bias), out_at, h.data_ptr(), n, *rest, tile_rows, act, ldx, _ld(w), ldo, _s(), _pdl())
+        native.call("prism_adapter_linear", x_at, w.data_ptr(), pool.a.data_ptr(), pool.b.data_ptr(), pool.scale.data_ptr(), pool.ranks.data_ptr(), index_at,
+                    lists_at, counts_at, _p(bias), out_at, h.data_ptr(), n, *rest, tile_rows, act, ldx, _ld(w), ldo, _s(), _pdl())
         x_at, out_at, index_at = x_at + 2 * n * ldx, out_at + 2 * n * ldo, index_at + 4 * n
         lists_at, counts_at, T = lists_at + 4 * run * capacity, counts_at + 4 * run, T - n
     return out
